@@ -191,6 +191,121 @@ int kf_optimized_attention_static(const void* q, const void* k, const void* v, c
  * recovers from it. */
 int kf_selftest_wait_timeout(int* status, long long limit_clocks, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Serving: rows in a paged key-value cache, and the attention of one new token
+ * per sequence over it.
+ *
+ * The cache is two pools of pages, K and V, [n_pages, Hkv, page_size, D] with D
+ * contiguous; row p of sequence b lies in row p % page_size of page
+ * pages[b * pages_stride + p / page_size].  Pages may be shared between
+ * sequences that only read them; table entries behind a sequence's rows are
+ * not looked at.  page_size is a multiple of 16.  The pools hold the dtype of
+ * q/k/v, or KF_E4M3: a row is then D e4m3 values times one power of two, whose
+ * exponent byte (e8m0) lies in [n_pages, Hkv, page_size] beside the pool: the
+ * smallest e >= -126 with largest magnitude <= 448 * 2^e (at most 119: larger
+ * magnitudes become 448 * 2^119).  A row that holds a value that
+ * is not finite has the NaN scale and reads back as NaN.
+ *
+ * Strides are in ELEMENTS of their tensor; those of q/k/v/out and the 16-bit
+ * pools are multiples of 8, those of e4m3 pools and of scales multiples of 16,
+ * base pointers 16-byte aligned.  Each struct below holds 8-byte fields only.
+ *
+ * K rows and queries go through RMSNorm (gamma; NULL: none) and the split-half
+ * rotation (cos/sin [n_positions, D]; NULL for both: none) in 32 bits and are
+ * rounded once, to the cache's type (K) or the type of the products (Q).
+ *
+ * What the lengths and tables on the device hold cannot be checked on the
+ * host.  A kernel that meets a table entry outside the cache writes 911 into
+ * the status word, a length or position that the table cannot hold 912, one
+ * behind the rotary tables 913; it never reads or writes out of bounds then, and
+ * what the call wrote is not to be trusted.  As everywhere, while the word is
+ * not 0 each call that is given it returns at once and writes nothing. */
+#define KF_E4M3 2
+
+#define KF_STATUS_BAD_PAGE 911
+#define KF_STATUS_BAD_LENGTH 912
+#define KF_STATUS_BAD_POSITION 913
+
+typedef struct kf_paged_cache {
+    void* k;                    /* [n_pages, Hkv, page_size, D] */
+    void* v;
+    void* k_scale;              /* [n_pages, Hkv, page_size], KF_E4M3 only */
+    void* v_scale;
+    const int32_t* pages;       /* [B, max_pages] */
+    int64_t pages_stride;       /* between the rows of `pages`; may be 0 */
+    int64_t n_pages, max_pages, page_size;
+    int64_t Hkv, D;
+    int64_t dtype;              /* KF_BF16, KF_FP16 or KF_E4M3 */
+    int64_t k_stride_page, k_stride_head, k_stride_row;
+    int64_t v_stride_page, v_stride_head, v_stride_row;
+    int64_t k_scale_stride_page, k_scale_stride_head;
+    int64_t v_scale_stride_page, v_scale_stride_head;
+} kf_paged_cache;
+
+/* Rows s < counts[b] of k, v [B, Hkv, S, D] to positions start[b] + s of
+ * sequence b (counts NULL: all S).  No row of the cache may be the target of
+ * two rows of one call. */
+typedef struct kf_append_params {
+    kf_paged_cache cache;
+    const void* k;
+    const void* v;
+    const void* gamma;          /* [D] or NULL */
+    const void* cos_table;      /* [n_positions, D] or NULL */
+    const void* sin_table;
+    const int32_t* start;       /* [B] */
+    const int32_t* counts;      /* [B] or NULL */
+    int* status;
+    int64_t B, S, dtype, n_positions;
+    int64_t k_stride_b, k_stride_h, k_stride_s;
+    int64_t v_stride_b, v_stride_h, v_stride_s;
+    double eps;
+} kf_append_params;
+int kf_append_rows(const kf_append_params* p, void* stream);
+
+/* Rows 0 .. lengths[b]-1 of every sequence to k, v [B, Hkv, S, D] of type
+ * `dtype` (KF_BF16 or KF_FP16; the cache's own if that is 16-bit); rows from
+ * lengths[b] to S-1 are written as zeros, rows of the cache from S on left out. */
+typedef struct kf_read_params {
+    kf_paged_cache cache;
+    void* k;
+    void* v;
+    const int32_t* lengths;     /* [B] */
+    int* status;
+    int64_t B, S, dtype;
+    int64_t k_stride_b, k_stride_h, k_stride_s;
+    int64_t v_stride_b, v_stride_h, v_stride_s;
+} kf_read_params;
+int kf_read_rows(const kf_read_params* p, void* stream);
+
+/* out[b, h] = softmax(scale * q'[b, h] K^T) V over the lengths[b] cached rows of
+ * sequence b, KV head h / (Hq / Hkv); q' is q normed and rotated at position
+ * lengths[b] - 1.  q, out [B, Hq, D].  Sequences with lengths[b] <= 0 get zeros.
+ * new_k, new_v (both or neither) [B, Hkv, D]: the newest token's rows, not in the
+ * cache yet; they are appended first, at position lengths[b] - 1 (K with gamma_k
+ * and the tables), for sequences with lengths[b] > 0.
+ * workspace: kf_decode_workspace_bytes() bytes of device memory, 16-byte
+ * aligned, that no other call uses until this one is done; need not be cleared. */
+typedef struct kf_decode_params {
+    kf_paged_cache cache;
+    const void* q;
+    const void* gamma_q;        /* [D] or NULL */
+    const void* cos_table;      /* [n_positions, D] or NULL */
+    const void* sin_table;
+    void* out;
+    const int32_t* lengths;     /* [B] */
+    const void* new_k;          /* NULL: only attention */
+    const void* new_v;
+    const void* gamma_k;        /* [D] or NULL */
+    void* workspace;
+    int* status;
+    int64_t B, Hq, dtype, n_positions;
+    int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h;
+    int64_t k_stride_b, k_stride_h, v_stride_b, v_stride_h;  /* of new_k, new_v */
+    double eps, scale;
+} kf_decode_params;
+size_t kf_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cache_dtype);
+int kf_decode_attention(const kf_decode_params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

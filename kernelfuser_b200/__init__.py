@@ -4,8 +4,11 @@ from .api import (KernelStatusError, attention_forward, attention_full, check_st
                   fused, launch_attention,
                   optimized_attention, optimized_attention_host, optimized_attention_static,
                   prepare_rows, release_host_pipelines, selftest_wait_timeout, status_word)
+from .cache import (PagedCache, append_rows, decode_attention, decode_step, decode_workspace_bytes,  # noqa: F401
+                    read_rows)
 from .inputs import WORKLOADS, Workload, make_inputs, make_workload_inputs, rope_tables  # noqa: F401
 
 __all__ = ["optimized_attention", "optimized_attention_host", "optimized_attention_static", "factored_attention", "fused", "prepare_rows", "attention_forward", "attention_full", "launch_attention", "check_status",
            "status_word", "KernelStatusError", "selftest_wait_timeout", "release_host_pipelines", "make_inputs", "make_workload_inputs", "rope_tables",
-           "WORKLOADS", "Workload"]
+           "WORKLOADS", "Workload",
+           "PagedCache", "append_rows", "read_rows", "decode_attention", "decode_step", "decode_workspace_bytes"]

@@ -14,10 +14,11 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libkf_b200.so"
 
-KF_BF16, KF_FP16 = 0, 1
+KF_BF16, KF_FP16, KF_E4M3 = 0, 1, 2
 EXPORTS = ("kf_version", "kf_last_error", "kf_prepare_rows", "kf_attention_fwd",
            "kf_static_scratch_bytes", "kf_optimized_attention_static", "kf_factored_attention",
-           "kf_selftest_wait_timeout", "kf_optimized_attention", "kf_attention_full")
+           "kf_selftest_wait_timeout", "kf_optimized_attention", "kf_attention_full",
+           "kf_append_rows", "kf_read_rows", "kf_decode_attention", "kf_decode_workspace_bytes")
 
 _lib = None
 
@@ -52,6 +53,12 @@ def _declare(lib):
                                            [c_void_p, c_int, c_void_p])
     lib.kf_selftest_wait_timeout.restype = c_int
     lib.kf_selftest_wait_timeout.argtypes = [c_void_p, ctypes.c_longlong, c_void_p]
+    # the serving operators take one struct of 8-byte fields (kernelfuser_b200.cache packs it) and the stream
+    for name in ("kf_append_rows", "kf_read_rows", "kf_decode_attention"):
+        getattr(lib, name).restype = c_int
+        getattr(lib, name).argtypes = [c_char_p, c_void_p]
+    lib.kf_decode_workspace_bytes.restype = ctypes.c_size_t
+    lib.kf_decode_workspace_bytes.argtypes = [c_int64] * 5
     return lib
 
 

@@ -34,7 +34,11 @@ def _default_variant() -> int:
 
 
 class KernelStatusError(RuntimeError):
-    """A kernel gave up on a bounded wait and reported a status code."""
+    """A kernel gave up on a bounded wait, or met an index that its tensors cannot hold, and reported a status code."""
+
+
+_STATUS_MEANS = {911: "a page table entry is outside the cache", 912: "a length or position is outside the page table",
+                 913: "a position is behind the rotary tables"}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
@@ -54,7 +58,7 @@ def check_status(device=None) -> None:
     code = int(w.item())
     if code != 0:
         w.zero_()
-        raise KernelStatusError(f"kernel reported status {code} (a bounded wait expired)")
+        raise KernelStatusError(f"kernel reported status {code} ({_STATUS_MEANS.get(code, 'a bounded wait expired')})")
 
 
 def selftest_wait_timeout(limit_clocks: int = 100_000, device=None) -> None:

@@ -18,7 +18,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libkf_b200.so"
 STAMP = PKG / "libkf_b200.srchash"  # content hash of the sources the library was built from
-SOURCES = [CSRC / "kf_api.cu"]
+SOURCES = [CSRC / "kf_api.cu", CSRC / "kf_cache.cu"]
 
 
 def _nvcc() -> str:
@@ -56,7 +56,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     cmd = [_nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O3", "-lineinfo",
            "-Xcompiler", "-fPIC", "-shared",
-           "-Xptxas", "-v" if verbose else "-warn-spills",
+           "-Xptxas", "-v" if verbose else "-warn-spills", "--threads", "0",
            "-o", str(LIB)] + [str(s) for s in SOURCES]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:

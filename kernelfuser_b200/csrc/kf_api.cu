@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/kf_b200.h"
+#include "host.cuh"
 #include "attn_fwd_basic.cuh"
 #include "attn_fwd_ws.cuh"
 #include "attn_fwd_persist.cuh"
@@ -31,102 +32,9 @@ extern "C" int kf_debug_time(long long* host_out) {
 }
 #endif
 
+using namespace kf::host;
+
 namespace {
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-// `dependent`: launch as a programmatic dependent of the kernel before it in the stream (the grid may start while
-// that kernel still runs and must order its reads of that kernel's output with griddepcontrol.wait).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_kernel_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool dependent,
-                             Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    if (dependent) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-    }
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-template <typename... KArgs, typename... Args>
-cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
-    return launch_kernel_ex(kern, grid, block, smem, st, false, std::forward<Args>(args)...);
-}
-
-// Identity of the calling thread's CUDA context: never used again in a process, and a new one after a device reset.
-// 0: unknown (no context yet), to be treated as one never seen.
-unsigned long long context_id() {
-    using Fn = CUresult (*)(CUcontext, unsigned long long*);
-    static std::atomic<Fn> cached{nullptr};
-    Fn fn = cached.load(std::memory_order_acquire);
-    if (fn == nullptr) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuCtxGetId", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-            return 0;
-        fn = reinterpret_cast<Fn>(p);
-        cached.store(fn, std::memory_order_release);
-    }
-    unsigned long long id = 0;
-    return fn(nullptr, &id) == CUDA_SUCCESS ? id : 0;
-}
-
-// Let a kernel use `bytes` of dynamic shared memory.  The setting belongs to the context: made at the kernel's first
-// launch in each (0.6 us).
-template <auto KERN> cudaError_t allow_smem(int bytes) {
-    static std::atomic<unsigned long long> done[64];  // contexts by id (two threads may both set it)
-    const unsigned long long id = context_id();
-    if (id != 0 && done[id % 64].load(std::memory_order_acquire) == id) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done[id % 64].store(id, std::memory_order_release);
-    return e;
-}
-
-// Device address, in the current context, of a variable of the library image; looked up once per context.
-struct SymbolCache {
-    std::atomic_flag busy = ATOMIC_FLAG_INIT;
-    unsigned long long id[64];
-    void* at[64];
-};
-cudaError_t symbol_address(SymbolCache& c, const void* symbol, void** out) {
-    const unsigned long long id = context_id();
-    const int i = static_cast<int>(id % 64);
-    auto locked = [&](auto&& body) {
-        while (c.busy.test_and_set(std::memory_order_acquire)) {}
-        body();
-        c.busy.clear(std::memory_order_release);
-    };
-    void* p = nullptr;
-    locked([&] { if (id != 0 && c.id[i] == id) p = c.at[i]; });
-    if (p == nullptr) {
-        cudaError_t e = cudaGetSymbolAddress(&p, symbol);
-        if (e != cudaSuccess) return e;
-        if (const unsigned long long now = context_id())  // (the call may have made the context)
-            locked([&] { c.id[now % 64] = now; c.at[now % 64] = p; });
-    }
-    *out = p;
-    return cudaSuccess;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-// Element stride of a dimension of extent n: a multiple of 8 (16 bytes), positive unless the dimension has a
-// single entry.  A zero stride over n > 1 entries (an expanded / broadcast view) is refused: the TMA maps
-// describe distinct rows and would walk past the allocation.
-bool stride_ok(int64_t s, int64_t n) { return (s % 8) == 0 && (s > 0 || (s == 0 && n == 1)); }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -193,21 +101,6 @@ int make_map(CUtensorMap* m, const void* base, int dtype, int B, int H, int S, i
     g_maps.key[slot] = k;
     g_maps.map[slot] = *m;
     g_maps.used[slot] = true;
-    return KF_OK;
-}
-
-int check_device() {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return fail(KF_ECUDA, "cudaGetDevice failed");
-    static int cached_major[64];
-    if (dev < 0 || dev >= 64) return fail(KF_ECUDA, "device ordinal %d out of range", dev);
-    if (cached_major[dev] == 0) {
-        int major = 0;
-        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-            return fail(KF_ECUDA, "cannot query the compute capability");
-        cached_major[dev] = major;
-    }
-    if (cached_major[dev] != 10) return fail(KF_ENOSUP, "this library is built for sm_100a (compute capability 10.x)");
     return KF_OK;
 }
 
@@ -313,18 +206,6 @@ constexpr long long kPair256MinSubBlocksPerSm = 85;
 constexpr long long kAutoPersistMinSubBlocksPerSm = 2000;
 constexpr long long kAutoPersistMinTiles = 8192;
 constexpr int kAutoPersistMinS = 2048, kAutoPersistMaxS = 8192;
-
-int sm_count() {
-    static int cached[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (cached[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-        cached[dev] = n;
-    }
-    return cached[dev];
-}
 
 // Work counters of the persistent kernels: {next item, CTAs that have left}, zero between launches (in the library image;
 // the last CTA of a launch puts them back).  Launches into a stream take the first kSchedSlots in turn, so two could only
