@@ -12,14 +12,19 @@
 // at most two broken ones; a broken item's pieces meet in the workspace and are joined by decode_join_kernel.
 //
 // Inside a CTA each of the four warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
-// into its own ring in shared memory (cp.async, across item borders), and keeps its own running maximum, sum and output;
-// the four meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are the m16 of
-// mma.m16n8k16 and the query heads its n8, so up to eight heads cost one instruction per 16 x 16 block of the cache.
-// (The 128-row MMAs of the prefill kernels have nothing to fill their rows with here.)
-// Rounding: q' and the probabilities are rounded to the 16-bit type of the product they enter; scores, maxima, sums and
-// outputs are 32 bits.  An e4m3 cache is widened to f16 (exact) on the way into the product; q' is scaled there by a power
-// of two per head so that its largest value is between 2^14 and 2^15; a key's scale multiplies its score, and a value row's scale
-// goes into the exponent of its probability, whose running maximum for O is kept apart from the one for the sum.
+// into its own ring of slots in shared memory (cp.async, across item borders), and keeps its own sum and output; the four
+// meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are the m16 of mma.m16n8k16 and the
+// query heads its n8, so up to eight heads cost one instruction per 16 x 16 block of the cache.  (The 128-row MMAs of the
+// prefill kernels have nothing to fill their rows with here.)  Q is prepared once per item, a row to a warp, from values
+// that are loaded while the item before is computed.
+// The exponentials are taken against a base that is only moved when a score exceeds it by more than 2^8 (exact after the
+// division by the sum): as a rule no lane waits for a maximum over lanes.
+// Rounding: q' and the probabilities enter the products as the sum of two 16-bit numbers, so that what is left of them is
+// 2^-16 (bf16) or 2^-22 (fp16) of each: a single rounding there doubled the error of a bf16 result (1.6e-3 -> 3.1e-3
+// relative), and the products wait for HBM anyway.  Scores, sums and outputs are 32 bits.  An e4m3 cache is widened to f16
+// (exact) on the way into the product; q' is scaled there by a power of two per head so that its largest value is between
+// 2^14 and 2^15; a key's scale multiplies its score, and a value row's scale goes into the exponent of its probability,
+// whose base for O is kept apart from the one for the sum.
 #pragma once
 #include <type_traits>
 
@@ -46,18 +51,20 @@ constexpr int kDecUnit = kDecKeys * kDecWarps;  // keys of a unit
 constexpr int kDecMinUnits = 4;                 // a CTA's piece is at least this long
 
 template <int D, bool E8, int NT> struct DecodeCfg {
-    static constexpr int kRowBytes = D * (E8 ? 1 : 2);
-    static constexpr int kTileBytes = kDecKeys * kRowBytes;  // K or V of a step
-    static constexpr int kScaleBytes = E8 ? 2 * kDecKeys : 0;
-    static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
-    static constexpr int kCtasPerSm = D == 256 && !E8 ? 1 : 2;
-    static constexpr int kStages = kTileBytes == 2048 ? 6 : 3;
     static constexpr int kRows = 8 * NT;
-    static constexpr int kMergeCols = 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
-    static constexpr int kRingBytes = kDecWarps * kStages * kStageBytes;
-    static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + 2 * kDecWarps * kRows * 4;
-    static constexpr int kSmemBytes = kRingBytes + kMergeBytes;
-    static constexpr int kPartFloats = kRows * D + 2 * kRows;  // output, maximum, sum of a broken item
+    static constexpr int kRowBytes = D * (E8 ? 1 : 2);
+    static constexpr int kTileBytes = kDecKeys * kRowBytes;           // K or V rows of a step
+    static constexpr int kSlotBytes = kTileBytes + (E8 ? kDecKeys : 0);  // and their scales
+    static constexpr bool kQueryInRegs = D * NT <= 256;               // else its fragments are read for every step
+    static constexpr int kCtasPerSm = kQueryInRegs ? 2 : 1;
+    // slots of a warp's ring: 100 KB in flight per CTA, as far as two of them fit an SM
+    static constexpr int kSlots = E8 ? (D == 128 ? 10 : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
+    static constexpr int kMergeCols = 128, kPad = kMergeCols + 4;     // columns that meet at a time; a row in shared memory
+    static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
+    static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
+    static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kDecWarps + 1) * kRows * 4;
+    static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes;
+    static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
@@ -112,90 +119,143 @@ struct DecodeCursor {
     }
 };
 
-// The 16-bit fragments of a row block's query heads.  Lane l holds row l/4 of each n8 block; the columns are those that a
-// K fragment of the same step has: of 16 columns 2t, 2t+1, 2t+8, 2t+9 (16-bit cache) or 4t .. 4t+3 (8-bit), t = l%4.
-// A column and its rotation partner D/2 further are in the same lane.  Returns what the row's scores are to be multiplied
-// with to undo the scaling of its values.
-template <int D, typename T, bool E8>
-__device__ __forceinline__ float query_fragment(const DecodeArgs& a, int b, int head, bool valid, int pos, uint32_t (&f)[D / 16][2]) {
-    constexpr int N = D / 4;  // values a lane holds
-    const int t = threadIdx.x % 4;
-    float x[N];
-    auto load = [&](const void* p, float (&y)[N]) {
-        const T* const base = reinterpret_cast<const T*>(p);
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            uint32_t w[2];
-            if constexpr (E8) {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(base + 16 * j) + t);
-                w[0] = u.x;
-                w[1] = u.y;
-            } else {
-                w[0] = __ldg(reinterpret_cast<const uint32_t*>(base + 16 * j) + t);
-                w[1] = __ldg(reinterpret_cast<const uint32_t*>(base + 16 * j + 8) + t);
-            }
-            const float2 u0 = Num<T>::unpack(w[0]), u1 = Num<T>::unpack(w[1]);
-            y[4 * j] = u0.x;
-            y[4 * j + 1] = u0.y;
-            y[4 * j + 2] = u1.x;
-            y[4 * j + 3] = u1.y;
-        }
+// Two values, each as high + low of the products' type: high is rounded towards zero, so that low has the value's sign and
+// together they hold twice the type's bits.  A low part that would be zero becomes the type's smallest number instead
+// (kMin, far below what is kept): an infinity in the cache then meets two factors of one sign and stays that infinity.
+template <typename M> struct Split;
+template <> struct Split<__nv_bfloat16> {
+    static constexpr float kMin = 0x1p-126f;
+    __device__ static __forceinline__ uint32_t toward_zero(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+template <> struct Split<__half> {
+    static constexpr float kMin = 0x1p-24f;
+    __device__ static __forceinline__ uint32_t toward_zero(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+};
+// values of any sign (a zero stays zero in both parts)
+template <typename M> __device__ __forceinline__ void split2(float x, float y, uint32_t& high, uint32_t& low) {
+    high = Split<M>::toward_zero(x, y);
+    const float2 h = Num<M>::unpack(high);
+    auto rest = [](float v, float hv) {
+        const float r = v - hv;
+        return fabsf(r) < Split<M>::kMin && v != 0.f ? copysignf(Split<M>::kMin, v) : r;
     };
-    if (valid) {
-        load(reinterpret_cast<const T*>(a.q) + b * a.q_sb + head * a.q_sh, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = 0.f;
-    }
-    if (a.gamma != nullptr) {
-        float ss = 0.f, g[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
-        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-        ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-        const float inv = rsqrtf(ss * (1.0f / static_cast<float>(D)) + a.eps);
-        load(a.gamma, g);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = x[i] * inv * g[i];
-    }
-    if (a.cos != nullptr && pos < a.n_pos) {
-        float c[N], s[N];
-        load(reinterpret_cast<const T*>(a.cos) + static_cast<long long>(pos) * D, c);
-        load(reinterpret_cast<const T*>(a.sin) + static_cast<long long>(pos) * D, s);
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-            const float lo = x[i], hi = x[i + N / 2];
-            x[i] = lo * c[i] - hi * s[i];
-            x[i + N / 2] = hi * c[i + N / 2] + lo * s[i + N / 2];
-        }
-    }
-    float back = 1.f;
-    if constexpr (E8) {
-        uint32_t amax = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // largest value to [2^14, 2^15) (an infinity or a NaN stays what it is)
-        const uint32_t e = min(max(amax >> 23, 15u), 254u);
-        const float up = __uint_as_float((268u - e) << 23);  // 2^(141 - e)
-        back = __uint_as_float((e - 14u) << 23);             // 2^(e - 141)
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] *= up;
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            f[j][0] = Num<__half>::pack(x[4 * j], x[4 * j + 1]);
-            f[j][1] = Num<__half>::pack(x[4 * j + 2], x[4 * j + 3]);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            f[j][0] = Num<T>::pack(x[4 * j], x[4 * j + 1]);
-            f[j][1] = Num<T>::pack(x[4 * j + 2], x[4 * j + 3]);
-        }
-    }
-    return back;
+    low = Num<M>::pack(rest(x, h.x), rest(y, h.y));
 }
+// probabilities; FLOOR: against infinities in the cache (an 8-bit one has none)
+template <typename M, bool FLOOR> __device__ __forceinline__ void split2_probabilities(float x, float y, uint32_t& high, uint32_t& low) {
+    if constexpr (FLOOR) {  // (x < kMin and not max(): a NaN stays one)
+        x = x < Split<M>::kMin ? Split<M>::kMin : x;
+        y = y < Split<M>::kMin ? Split<M>::kMin : y;
+    }
+    high = Split<M>::toward_zero(x, y);
+    const float2 h = Num<M>::unpack(high);
+    x -= h.x;
+    y -= h.y;
+    low = FLOOR ? Num<M>::pack(fmaxf(x, Split<M>::kMin), fmaxf(y, Split<M>::kMin)) : Num<M>::pack(x, y);
+}
+
+// The query rows that a warp prepares for an item (row, row + 4, ...: every lane holds the pairs of columns 2 lane + 64 p
+// and their rotation partners), loaded ahead of time.
+template <int D, typename T, int NT> struct QueryRows {
+    static constexpr int kPairs = D / 64, kN = 2 * NT;  // pairs of a lane and row; rows of a warp
+    uint32_t q[kN][kPairs], c[kPairs], s[kPairs];
+    __device__ __forceinline__ void load(const DecodeArgs& a, int b, int hk, int len) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = hk / a.row_blocks;
+        const int row0 = (hk - h * a.row_blocks) * 8 * NT;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const int r = row0 + warp + 4 * i;
+            const uint32_t* const src = reinterpret_cast<const uint32_t*>(
+                reinterpret_cast<const T*>(a.q) + b * a.q_sb + (h * a.G + r) * a.q_sh) + lane;
+#pragma unroll
+            for (int p = 0; p < kPairs; ++p) q[i][p] = r < a.G ? __ldg(src + 32 * p) : 0u;
+        }
+        if (a.cos != nullptr) {
+            const long long at = static_cast<long long>(min(len, a.n_pos) - 1) * (D / 2) + lane;
+#pragma unroll
+            for (int p = 0; p < kPairs; ++p) {
+                c[p] = __ldg(reinterpret_cast<const uint32_t*>(a.cos) + at + 32 * p);
+                s[p] = __ldg(reinterpret_cast<const uint32_t*>(a.sin) + at + 32 * p);
+            }
+        }
+    }
+    // Norm, rotation, and the fragments of the products into shared memory: lane l of a fragment holds row l/4, and of 16
+    // columns 2t, 2t+1, 2t+8, 2t+9 (16-bit cache) or 4t .. 4t+3 (8-bit), t = l%4, as a K fragment of that step does.
+    // back[row]: what the row's scores are to be multiplied with to undo the scaling of its values (8-bit cache).
+    template <bool E8> __device__ __forceinline__ void prepare(const DecodeArgs& a, const uint32_t (&gamma)[kPairs], uint4* frag, float* back) const {
+        using M = typename std::conditional<E8, __half, T>::type;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            float x[kPairs][2];
+#pragma unroll
+            for (int p = 0; p < kPairs; ++p) {
+                const float2 v = Num<T>::unpack(q[i][p]);
+                x[p][0] = v.x;
+                x[p][1] = v.y;
+            }
+            if (a.gamma != nullptr) {
+                float ss = 0.f;
+#pragma unroll
+                for (int p = 0; p < kPairs; ++p) ss = fmaf(x[p][0], x[p][0], fmaf(x[p][1], x[p][1], ss));
+#pragma unroll
+                for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+                const float inv = rsqrtf(ss * (1.0f / static_cast<float>(D)) + a.eps);
+#pragma unroll
+                for (int p = 0; p < kPairs; ++p) {
+                    const float2 v = Num<T>::unpack(gamma[p]);
+                    x[p][0] = x[p][0] * inv * v.x;
+                    x[p][1] = x[p][1] * inv * v.y;
+                }
+            }
+            if (a.cos != nullptr) {
+#pragma unroll
+                for (int p = 0; p < kPairs / 2; ++p) {
+                    constexpr int kP = kPairs / 2;
+                    const float2 cl = Num<T>::unpack(c[p]), ch = Num<T>::unpack(c[p + kP]);
+                    const float2 sl = Num<T>::unpack(s[p]), sh = Num<T>::unpack(s[p + kP]);
+                    const float lo0 = x[p][0], lo1 = x[p][1], hi0 = x[p + kP][0], hi1 = x[p + kP][1];
+                    x[p][0] = lo0 * cl.x - hi0 * sl.x;
+                    x[p][1] = lo1 * cl.y - hi1 * sl.y;
+                    x[p + kP][0] = hi0 * ch.x + lo0 * sh.x;
+                    x[p + kP][1] = hi1 * ch.y + lo1 * sh.y;
+                }
+            }
+            const int r = warp + 4 * i;
+            if constexpr (E8) {
+                uint32_t amax = 0;
+#pragma unroll
+                for (int p = 0; p < kPairs; ++p)
+                    amax = max(amax, max(__float_as_uint(x[p][0]) & 0x7fffffffu, __float_as_uint(x[p][1]) & 0x7fffffffu));
+                amax = __reduce_max_sync(0xffffffffu, amax);
+                // largest value to [2^14, 2^15) (an infinity or a NaN stays what it is)
+                const uint32_t e = min(max(amax >> 23, 15u), 254u);
+                const float up = __uint_as_float((268u - e) << 23);                    // 2^(141 - e)
+                if (lane == 0) back[r] = a.scale_log2e * __uint_as_float((e - 14u) << 23);  // 2^(e - 141)
+#pragma unroll
+                for (int p = 0; p < kPairs; ++p) {
+                    x[p][0] *= up;
+                    x[p][1] *= up;
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < kPairs; ++p) {
+                const int col = 2 * lane + 64 * p, in = col % 16;
+                const int t = E8 ? in / 4 : in % 8 / 2, reg = E8 ? in % 4 / 2 : in / 8;
+                uint32_t* const dst = reinterpret_cast<uint32_t*>(frag + (r / 8 * (D / 16) + col / 16) * 32 + r % 8 * 4 + t);
+                split2<M>(x[p][0], x[p][1], dst[reg], dst[reg + 2]);
+            }
+        }
+    }
+};
 
 // Where the broken items' parts and what joins them lie in the workspace: for each CTA two parts (0: an item that began
 // in an earlier CTA, 1: one that begins here), then for each CTA {item that begins here and goes on, or -1; last CTA of it}.
@@ -284,89 +344,140 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     }
     cc.left = static_cast<int>(u1 - u0);
 
-    // ---- the warp's ring of stages: K rows, V rows (16-byte pieces xor-ed with the row so that eight rows of a column
-    // block lie in different banks), scales
-    const uint32_t ring = smem_u32(smem) + warp * C::kStages * C::kStageBytes;
-    DecodeCursor pc = cc;
-    int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
-    bool fresh = true;                           // the producer stands at an item whose pages it has not looked up
-    auto issue = [&](int stage) {
-        const int key0 = pc.t * kDecUnit + warp * kDecKeys;
-        if (fresh || pc.t - table_at >= 32) {
-            fresh = false;
-            table_at = pc.t;
-            const int key = (pc.t + lane) * kDecUnit + warp * kDecKeys;
-            my_page = 0;
-            if (pc.t + lane < pc.nt && key < pc.len) {
-                const int i = key / a.c.page_size;
-                my_row = key - i * a.c.page_size;
-                my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
-                if (static_cast<unsigned>(my_page) >= static_cast<unsigned>(a.c.n_pages)) {
-                    report(a.status, kStatusBadPage);
-                    my_page = -1;
-                }
-            }
-        }
-        const int page = __shfl_sync(0xffffffffu, my_page, pc.t - table_at);
-        const int row0 = __shfl_sync(0xffffffffu, my_row, pc.t - table_at);
-        if (key0 < pc.len) {
-            constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces == 0 ? 1 : 32 / kPieces;
-            const int h = pc.hk / a.row_blocks, piece16 = lane % kPieces, r0 = lane / kPieces;
-            const long long row = page < 0 ? 0 : row0 + r0, pg = page < 0 ? 0 : page;
-            const int rows = page < 0 ? 0 : min(kDecKeys, pc.len - key0);
-            const unsigned char* kp = a.c.k + pg * a.c.k_sp + h * a.c.k_sh + row * a.c.k_ss + piece16 * 16;
-            const unsigned char* vp = a.c.v + pg * a.c.v_sp + h * a.c.v_sh + row * a.c.v_ss + piece16 * 16;
-            const uint32_t base = ring + stage * C::kStageBytes;
+    // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
+    // eight rows of a column block lie in different banks), scales behind them
+    const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
+    uint4* const frag = reinterpret_cast<uint4*>(smem + C::kRingBytes);
+    float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes + C::kQueryBytes);  // two copies of [8][kPad]
+    float* const merge_m = merge_o + 2 * 8 * C::kPad;                                        // [warps][rows]
+    float* const merge_l = merge_m + kDecWarps * kRows;
+    float* const back = merge_l + kDecWarps * kRows;                                         // [rows]
+
+    QueryRows<D, T, NT> rows;
+    rows.load(a, cc.b, cc.hk, cc.len);
+    uint32_t gamma[D / 64];
+    if (a.gamma != nullptr) {
 #pragma unroll
-            for (int i = 0; i < kDecKeys / kRowsAtOnce; ++i) {
-                const int r = r0 + i * kRowsAtOnce;
-                const uint32_t at = base + r * C::kRowBytes + ((piece16 ^ (r & 7)) << 4);
-                cp_async16(at, kp + (r < rows ? i * kRowsAtOnce * a.c.k_ss : 0), r < rows);
-                cp_async16(at + C::kTileBytes, vp + (r < rows ? i * kRowsAtOnce * a.c.v_ss : 0), r < rows);
-            }
-            if constexpr (E8) {
-                // (all 16 scales: a page holds a multiple of 16 rows)
-                if (lane == 0) cp_async16(base + 2 * C::kTileBytes, a.c.k_scale + pg * a.c.ks_sp + h * a.c.ks_sh + (row - r0), page >= 0);
-                if (lane == 0) cp_async16(base + 2 * C::kTileBytes + kDecKeys, a.c.v_scale + pg * a.c.vs_sp + h * a.c.vs_sh + (row - r0), page >= 0);
-            }
-        }
-        ++pc.t;
-        --pc.left;
-        if (pc.t == pc.nt && pc.left > 0) {
-            pc.next_item(a, HK);
-            fresh = true;
-        }
-    };
-#pragma unroll
-    for (int s = 0; s < C::kStages - 1; ++s) {
-        if (pc.left > 0) issue(s);
-        cp_async_commit();
+        for (int p = 0; p < D / 64; ++p) gamma[p] = __ldg(reinterpret_cast<const uint32_t*>(a.gamma) + lane + 32 * p);
     }
 
-    float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes);  // two copies of [8][kPad]
-    float* const merge_m = merge_o + 2 * 8 * C::kPad;                       // [warps][rows]
-    float* const merge_l = merge_m + kDecWarps * kRows;
-    // ldmatrix: the row (key) of the stage and the 16-byte piece that this lane names
+    DecodeCursor pc = cc;
+    int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
+    int page = 0, row0_in_page = 0;              // of the unit that is being copied
+    bool fresh = true;                           // the producer stands at an item whose pages it has not looked up
+    constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces;
+    const int piece16 = lane % kPieces, r_lane = lane / kPieces;
+    // 16 rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
+    auto copy_rows = [&](int slot, const unsigned char* pool, long long sp, long long sh, long long ss, const unsigned char* scale,
+                         long long scale_sp, long long scale_sh) {
+        const int key0 = pc.t * kDecUnit + warp * kDecKeys;
+        if (key0 >= pc.len) return;
+        const int h = pc.hk / a.row_blocks, n = page < 0 ? 0 : min(kDecKeys, pc.len - key0);
+        const long long pg = max(page, 0);
+        const unsigned char* src = pool + pg * sp + h * sh + (row0_in_page + r_lane) * ss + piece16 * 16;
+        const uint32_t base = ring + slot * C::kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < kDecKeys / kRowsAtOnce; ++i) {
+            const int r = r_lane + i * kRowsAtOnce;
+            cp_async16(base + r * C::kRowBytes + ((piece16 ^ (r & 7)) << 4), src + (r < n ? i * kRowsAtOnce * ss : 0), r < n);
+        }
+        if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
+            if (lane == 0) cp_async16(base + C::kTileBytes, scale + pg * scale_sp + h * scale_sh + row0_in_page, page >= 0);
+        }
+    };
+    auto issue_k = [&](int slot) {
+        if (pc.left > 0) {
+            if (fresh || pc.t - table_at >= 32) {
+                fresh = false;
+                table_at = pc.t;
+                const int key = (pc.t + lane) * kDecUnit + warp * kDecKeys;
+                my_page = my_row = 0;
+                if (pc.t + lane < pc.nt && key < pc.len) {
+                    const int i = key / a.c.page_size;
+                    my_row = key - i * a.c.page_size;
+                    my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
+                    if (static_cast<unsigned>(my_page) >= static_cast<unsigned>(a.c.n_pages)) {
+                        report(a.status, kStatusBadPage);
+                        my_page = -1;
+                        my_row = 0;
+                    }
+                }
+            }
+            page = __shfl_sync(0xffffffffu, my_page, pc.t - table_at);
+            row0_in_page = __shfl_sync(0xffffffffu, my_row, pc.t - table_at);
+            copy_rows(slot, a.c.k, a.c.k_sp, a.c.k_sh, a.c.k_ss, a.c.k_scale, a.c.ks_sp, a.c.ks_sh);
+        }
+        cp_async_commit();
+    };
+    auto issue_v = [&](int slot) {
+        if (pc.left > 0) {
+            copy_rows(slot, a.c.v, a.c.v_sp, a.c.v_sh, a.c.v_ss, a.c.v_scale, a.c.vs_sp, a.c.vs_sh);
+            ++pc.t;
+            --pc.left;
+            if (pc.t == pc.nt && pc.left > 0) {
+                pc.next_item(a, HK);
+                fresh = true;
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < C::kSlots - 1; ++s) {
+        if (s % 2 == 0) issue_k(s);
+        else issue_v(s);
+    }
+    // A step's two halves: wait for the slot, refill the one before it, which all lanes are done with.
+    int slot = 0;
+    auto arrive = [&](auto v) {  // v: true for the V half
+        constexpr bool kIsV = decltype(v)::value;
+        cp_async_wait<C::kSlots - 2>();
+        __syncwarp();
+        const int freed = slot == 0 ? C::kSlots - 1 : slot - 1;
+        if constexpr ((C::kSlots % 2 == 1) != kIsV) issue_k(freed);
+        else issue_v(freed);
+    };
+    auto leave = [&] { slot = slot + 1 == C::kSlots ? 0 : slot + 1; };
+
+    rows.template prepare<E8>(a, gamma, frag, back);
+    __syncthreads();
+
+    // ldmatrix: the row (key) of the slot and the 16-byte piece that this lane names
     const int q8 = lane >> 3;
     const int k_row = (q8 & 1) * 8 + (lane & 7), k_piece = q8 >> 1;
     const int v_row = E8 ? k_row : (q8 >> 1) * 8 + (lane & 7), v_piece = E8 ? k_piece : (q8 & 1);
+    // Probabilities are 2^(score - base + kUp), the base at most kSlack behind the largest score so far: up to 2^15 in f16,
+    // whose smallest step is then 2^-35 of the largest probability, up to 2^8 in bf16.
+    constexpr bool kHalf = std::is_same<M, __half>::value;
+    constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : 0.f;
 
-    int stage = 0, continues = -1, last_cta = 0;
+    int continues = -1, last_cta = 0;
     while (cc.left > 0) {
         // ---- one item's part: units cc.t .. cc.t + n - 1
         const int n = min(cc.nt - cc.t, cc.left);
         if (n <= 0) break;
         const int h = cc.hk / a.row_blocks, row0 = (cc.hk - h * a.row_blocks) * kRows;
-        uint32_t qf[NT][kDT][2];
+        DecodeCursor nc = cc;  // the item after this one: its query rows are on their way meanwhile
+        nc.t += n;
+        nc.left -= n;
+        if (nc.left > 0) {
+            nc.next_item(a, HK);
+            rows.load(a, nc.b, nc.hk, nc.len);
+        }
+        uint4 qf[C::kQueryInRegs ? NT : 1][C::kQueryInRegs ? kDT : 1];
+        if constexpr (C::kQueryInRegs) {
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int j = 0; j < kDT; ++j) qf[u][j] = frag[(u * kDT + j) * 32 + lane];
+        }
         float mul[NT][2];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
-            const int r = row0 + u * 8 + g;
-            const float back = query_fragment<D, T, E8>(a, cc.b, h * a.G + r, r < a.G, cc.len - 1, qf[u]);
-            mul[u][0] = a.scale_log2e * __shfl_sync(0xffffffffu, back, 8 * t4);      // row 2 t4
-            mul[u][1] = a.scale_log2e * __shfl_sync(0xffffffffu, back, 8 * t4 + 4);  // row 2 t4 + 1
+            mul[u][0] = E8 ? back[u * 8 + 2 * t4] : a.scale_log2e;
+            mul[u][1] = E8 ? back[u * 8 + 2 * t4 + 1] : a.scale_log2e;
         }
-        float o[NT][kDT][4], m[NT][2], l[NT][2], mv[NT][2];  // mv: reference of O (its own only for an 8-bit cache)
+        // m, mv: bases of the sum and of O (an 8-bit cache's value scales belong to the latter), -inf before the first key
+        float o[NT][kDT][4], m[NT][2], mv[NT][2], l[NT][2];
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
 #pragma unroll
@@ -375,20 +486,26 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             l[u][0] = l[u][1] = 0.f;
         }
         for (int i_unit = 0; i_unit < n; ++i_unit) {
-            cp_async_wait<C::kStages - 2>();
-            __syncwarp();  // all lanes' copies of this stage are there, and all lanes are done with the stage before it
-            {
-                const int next = stage == 0 ? C::kStages - 1 : stage - 1;
-                if (pc.left > 0) issue(next);
-                cp_async_commit();
-            }
             const int key0 = (cc.t + i_unit) * kDecUnit + warp * kDecKeys;
-            if (key0 < cc.len) {
-                const uint32_t ks = ring + stage * C::kStageBytes, vs = ks + C::kTileBytes;
-                // S^T: keys g, g + 8 (rows), heads 2 t4, 2 t4 + 1 (columns)
-                float s[NT][4];
+            const bool work = key0 < cc.len;
+            arrive(std::false_type{});
+            float x[NT][4], w[NT][4];  // scores of keys g (0, 1), g + 8 (2, 3) and heads 2 t4, 2 t4 + 1
+            float ks0 = 1.f, ks1 = 1.f;
+            if (work) {
+                const uint32_t ks = ring + slot * C::kSlotBytes;
+                float s[NT][2][4];  // high and low part of q': two chains of products
 #pragma unroll
-                for (int u = 0; u < NT; ++u) s[u][0] = s[u][1] = s[u][2] = s[u][3] = 0.f;
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[u][0][i] = s[u][1][i] = 0.f;
+                auto product = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        const uint4 f = C::kQueryInRegs ? qf[C::kQueryInRegs ? u : 0][C::kQueryInRegs ? j : 0] : frag[(u * kDT + j) * 32 + lane];
+                        mma16816<M>(s[u][0], a0, a1, a2, a3, f.x, f.y);
+                        mma16816<M>(s[u][1], a0, a1, a2, a3, f.z, f.w);
+                    }
+                };
                 const uint32_t k_at = ks + k_row * C::kRowBytes;
                 if constexpr (E8) {
 #pragma unroll
@@ -396,74 +513,97 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                         uint32_t r[4];
                         ldmatrix4(r, k_at + (((j + k_piece) ^ (k_row & 7)) << 4));
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t a0 = e4m3_to_half2(r[2 * x]), a2 = e4m3_to_half2(r[2 * x] >> 16);
-                            const uint32_t a1 = e4m3_to_half2(r[2 * x + 1]), a3 = e4m3_to_half2(r[2 * x + 1] >> 16);
-#pragma unroll
-                            for (int u = 0; u < NT; ++u) mma16816<M>(s[u], a0, a1, a2, a3, qf[u][j + x][0], qf[u][j + x][1]);
-                        }
+                        for (int y = 0; y < 2; ++y)
+                            product(j + y, e4m3_to_half2(r[2 * y]), e4m3_to_half2(r[2 * y + 1]), e4m3_to_half2(r[2 * y] >> 16),
+                                    e4m3_to_half2(r[2 * y + 1] >> 16));
                     }
+                    const unsigned char* sc = smem + (warp * C::kSlots + slot) * C::kSlotBytes + C::kTileBytes;
+                    ks0 = scale_value(sc[g]);
+                    ks1 = scale_value(sc[g + 8]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < kDT; ++j) {
                         uint32_t r[4];
                         ldmatrix4(r, k_at + (((2 * j + k_piece) ^ (k_row & 7)) << 4));
-#pragma unroll
-                        for (int u = 0; u < NT; ++u) mma16816<M>(s[u], r[0], r[1], r[2], r[3], qf[u][j][0], qf[u][j][1]);
+                        product(j, r[0], r[1], r[2], r[3]);
                     }
                 }
                 const bool in0 = key0 + g < cc.len, in1 = key0 + g + 8 < cc.len;
-                float ks0 = 1.f, ks1 = 1.f, ve0 = 0.f, ve1 = 0.f;  // factors of the keys, exponents of the value rows
-                if constexpr (E8) {
-                    const unsigned char* sc = smem + (vs + C::kTileBytes - smem_u32(smem));
-                    ks0 = scale_value(sc[g]);
-                    ks1 = scale_value(sc[g + 8]);
-                    ve0 = sc[16 + g] == 255 ? NAN : static_cast<float>(sc[16 + g]) - 127.f;
-                    ve1 = sc[24 + g] == 255 ? NAN : static_cast<float>(sc[24 + g]) - 127.f;
-                }
-                uint32_t pb[NT][2];
 #pragma unroll
-                for (int u = 0; u < NT; ++u) {
-                    float x[4], w[4];
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[u][i] = (i < 2 ? in0 : in1) ? (s[u][0][i] + s[u][1][i]) * mul[u][i & 1] * (i < 2 ? ks0 : ks1) : -INFINITY;
+            }
+            leave();
+            arrive(std::true_type{});
+            if (work) {
+                const uint32_t vs = ring + slot * C::kSlotBytes;
+                float ve0 = 0.f, ve1 = 0.f;  // exponents of the value rows
+                if constexpr (E8) {
+                    const unsigned char* sc = smem + (warp * C::kSlots + slot) * C::kSlotBytes + C::kTileBytes;
+                    ve0 = sc[g] == 255 ? NAN : static_cast<float>(sc[g]) - 127.f;
+                    ve1 = sc[g + 8] == 255 ? NAN : static_cast<float>(sc[g + 8]) - 127.f;
+                }
+                bool above = false;
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[i] = (i < 2 ? in0 : in1) ? s[u][i] * mul[u][i & 1] * (i < 2 ? ks0 : ks1) : -INFINITY;
-                        w[i] = E8 ? ((i < 2 ? in0 : in1) ? x[i] + (i < 2 ? ve0 : ve1) : -INFINITY) : x[i];
-                    }
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float mx = fmaxf(x[c], x[c + 2]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(m[u][c], fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)));
-                        const float base = mx == -INFINITY ? 0.f : mx;
-                        l[u][c] = l[u][c] * ex2(m[u][c] - base) + (ex2(x[c] - base) + ex2(x[c + 2] - base));
-                        m[u][c] = mx;
-                        float base_v = base;
-                        float from = mv[u][c];
+                        w[u][i] = x[u][i];
+                        above |= x[u][i] > m[u][i & 1] + kSlack;
                         if constexpr (E8) {
-                            float my = fmaxf(w[c], w[c + 2]);
-                            my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 4));
-                            my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 8));
-                            mx = fmaxf(from, fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 16)));
-                            base_v = mx == -INFINITY ? 0.f : mx;
+                            w[u][i] = x[u][i] == -INFINITY ? x[u][i] : x[u][i] + (i < 2 ? ve0 : ve1);
+                            above |= w[u][i] > mv[u][i & 1] + kSlack;
                         }
-                        mv[u][c] = mx;
-                        if (__any_sync(0xffffffffu, from != mx)) {
-                            const float f = ex2(from - base_v);
+                    }
+                if (__any_sync(0xffffffffu, above)) {  // move the bases to the maxima so far
+                    auto top = [](float y, float z, float so_far) {
+                        y = fmaxf(y, z);
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                        return fmaxf(so_far, fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16)));
+                    };
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const float to = top(x[u][c], x[u][c + 2], m[u][c]);
+                            const float to_v = E8 ? top(w[u][c], w[u][c + 2], mv[u][c]) : to;
+                            l[u][c] *= m[u][c] == -INFINITY ? 0.f : ex2(m[u][c] - to);
+                            const float f = mv[u][c] == -INFINITY ? 0.f : ex2(mv[u][c] - to_v);
 #pragma unroll
                             for (int i = 0; i < kDT; ++i) {
                                 o[u][i][c] *= f;
                                 o[u][i][c + 2] *= f;
                             }
+                            m[u][c] = to;
+                            mv[u][c] = to_v;
                         }
-                        w[c] = ex2(w[c] - base_v);
-                        w[c + 2] = ex2(w[c + 2] - base_v);
-                    }
-                    pb[u][0] = transpose8x8(Num<M>::pack(w[0], w[1]));
-                    pb[u][1] = transpose8x8(Num<M>::pack(w[2], w[3]));
                 }
-                // O^T += V^T P^T
+                uint32_t pb[NT][4];  // high and low part of the probabilities of keys 0-7, 8-15
+#pragma unroll
+                for (int u = 0; u < NT; ++u) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float base = m[u][c] == -INFINITY ? 0.f : m[u][c], base_v = mv[u][c] == -INFINITY ? 0.f : mv[u][c];
+                        const float p0 = ex2(x[u][c] - (base - kUp)), p1 = ex2(x[u][c + 2] - (base - kUp));
+                        l[u][c] += p0 + p1;
+                        w[u][c] = E8 ? ex2(w[u][c] - (base_v - kUp)) : p0;
+                        w[u][c + 2] = E8 ? ex2(w[u][c + 2] - (base_v - kUp)) : p1;
+                    }
+                    split2_probabilities<M, !E8>(w[u][0], w[u][1], pb[u][0], pb[u][2]);
+                    split2_probabilities<M, !E8>(w[u][2], w[u][3], pb[u][1], pb[u][3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) pb[u][i] = transpose8x8(pb[u][i]);
+                }
+                auto product = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+                        mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][2], pb[u][3]);
+                    }
+                };
                 const uint32_t v_at = vs + v_row * C::kRowBytes;
                 if constexpr (E8) {
 #pragma unroll
@@ -471,13 +611,10 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                         uint32_t r[4];
                         ldmatrix4_trans(r, v_at + (((i + v_piece) ^ (v_row & 7)) << 4));
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
+                        for (int y = 0; y < 2; ++y) {
                             // bytes {key 2t col 2g, key 2t col 2g+1, key 2t+1 col 2g, key 2t+1 col 2g+1}
-                            const uint32_t y0 = __byte_perm(r[2 * x], 0, 0x3120), y1 = __byte_perm(r[2 * x + 1], 0, 0x3120);
-                            const uint32_t a0 = e4m3_to_half2(y0), a1 = e4m3_to_half2(y0 >> 16);
-                            const uint32_t a2 = e4m3_to_half2(y1), a3 = e4m3_to_half2(y1 >> 16);
-#pragma unroll
-                            for (int u = 0; u < NT; ++u) mma16816<M>(o[u][i + x], a0, a1, a2, a3, pb[u][0], pb[u][1]);
+                            const uint32_t y0 = __byte_perm(r[2 * y], 0, 0x3120), y1 = __byte_perm(r[2 * y + 1], 0, 0x3120);
+                            product(i + y, e4m3_to_half2(y0), e4m3_to_half2(y0 >> 16), e4m3_to_half2(y1), e4m3_to_half2(y1 >> 16));
                         }
                     }
                 } else {
@@ -485,12 +622,11 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                     for (int i = 0; i < kDT; ++i) {
                         uint32_t r[4];
                         ldmatrix4_trans(r, v_at + (((2 * i + v_piece) ^ (v_row & 7)) << 4));
-#pragma unroll
-                        for (int u = 0; u < NT; ++u) mma16816<M>(o[u][i], r[0], r[1], r[2], r[3], pb[u][0], pb[u][1]);
+                        product(i, r[0], r[1], r[2], r[3]);
                     }
                 }
             }
-            stage = stage + 1 == C::kStages ? 0 : stage + 1;
+            leave();
         }
 
         // ---- the four warps' parts of the item together
@@ -545,6 +681,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 };
                 if (warp >= 2) each([&](int at, float x) { copy[at] = x; });
                 __syncthreads();
+                if (u == 0 && c0 == 0 && nc.left > 0) rows.template prepare<E8>(a, gamma, frag, back);  // (all are done with the old ones)
                 if (warp < 2) each([&](int at, float x) { copy[at] += x; });
                 __syncthreads();
                 for (int i = tid; i < 8 * (C::kMergeCols / 4); i += kDecThreads) {
@@ -575,9 +712,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 }
                 __syncthreads();  // the copies are free
             }
-        cc.t += n;
-        cc.left -= n;
-        if (cc.left > 0) cc.next_item(a, HK);
+        cc = nc;
     }
     cp_async_wait<0>();
     if (tid == 0) {
