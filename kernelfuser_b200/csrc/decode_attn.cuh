@@ -53,23 +53,27 @@ constexpr int kDecMinUnits = 4;                 // a CTA's piece is at least thi
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
     static constexpr int kRowBytes = D * (E8 ? 1 : 2);
-    static constexpr int kTileBytes = kDecKeys * kRowBytes;           // K or V rows of a step
-    static constexpr int kSlotBytes = kTileBytes + (E8 ? kDecKeys : 0);  // and their scales
+    static constexpr int kSlotBytes = kDecKeys * kRowBytes;           // K or V rows of a step
+    static constexpr int kScaleBytes = E8 ? kDecKeys : 0;             // and their scales
     static constexpr bool kQueryInRegs = D * NT <= 256;               // else its fragments are read for every step
     static constexpr int kCtasPerSm = kQueryInRegs ? 2 : 1;
-    // slots of a warp's ring: 100 KB in flight per CTA, as far as two of them fit an SM
+    // slots of a warp's ring: 100 KB per CTA, as far as two of them fit an SM
     static constexpr int kSlots = E8 ? (D == 128 ? 10 : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
     static constexpr int kMergeCols = 128, kPad = kMergeCols + 4;     // columns that meet at a time; a row in shared memory
     static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
+    static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
     static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kDecWarps + 1) * kRows * 4;
-    static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes;
+    static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
     const int n = take ? 16 : 0;  // (0: zeros, nothing is read)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -96,6 +100,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Four e4m3 as two f16x2 (exact).
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(x));
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -107,13 +115,15 @@ __device__ __forceinline__ int units_of(int len) { return (len + kDecUnit - 1) /
 
 // A place in the line of units: unit t of nt of item hk of sequence b.
 struct DecodeCursor {
-    int b, hk, t, nt, len;
+    int b, hk, h, t, nt, len;
     int left;  // units up to the end of the CTA's piece
     // to the next item; only called with units left
     __device__ __forceinline__ void next_item(const DecodeArgs& a, int HK) {
         t = 0;
-        if (++hk < HK) return;
-        hk = 0;
+        ++hk;
+        h = hk / a.row_blocks;
+        if (hk < HK) return;
+        hk = h = 0;
         do len = cached_rows(a, ++b); while (len == 0 && b + 1 < a.B);
         nt = units_of(len);
     }
@@ -271,7 +281,6 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     using C = DecodeCfg<D, E8, NT>;
     using M = typename std::conditional<E8, __half, T>::type;  // type of the products' operands
     constexpr int kDT = D / 16, kRows = C::kRows;
-    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ long long s_sum[kDecWarps], s_first;
     __shared__ int s_b, s_dead;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -341,12 +350,15 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         const long long in_b = u0 - s_first * HK;
         cc.hk = static_cast<int>(in_b / cc.nt);
         cc.t = static_cast<int>(in_b - static_cast<long long>(cc.hk) * cc.nt);
+        cc.h = cc.hk / a.row_blocks;
     }
     cc.left = static_cast<int>(u1 - u0);
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
-    // eight rows of a column block lie in different banks), scales behind them
+    // eight rows of a column block lie in different banks)
+    extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
+    unsigned char* const scales = smem + C::kSmemBytes - C::kScaleRingBytes + warp * C::kSlots * C::kScaleBytes;
     uint4* const frag = reinterpret_cast<uint4*>(smem + C::kRingBytes);
     float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes + C::kQueryBytes);  // two copies of [8][kPad]
     float* const merge_m = merge_o + 2 * 8 * C::kPad;                                        // [warps][rows]
@@ -365,24 +377,31 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
     int page = 0, row0_in_page = 0;              // of the unit that is being copied
     bool fresh = true;                           // the producer stands at an item whose pages it has not looked up
-    constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces;
+    constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kCopies = kDecKeys / kRowsAtOnce;
     const int piece16 = lane % kPieces, r_lane = lane / kPieces;
+    const uint32_t dst_lane = ring + r_lane * C::kRowBytes + ((piece16 ^ (r_lane & 7)) << 4);
     // 16 rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
     auto copy_rows = [&](int slot, const unsigned char* pool, long long sp, long long sh, long long ss, const unsigned char* scale,
                          long long scale_sp, long long scale_sh) {
-        const int key0 = pc.t * kDecUnit + warp * kDecKeys;
-        if (key0 >= pc.len) return;
-        const int h = pc.hk / a.row_blocks, n = page < 0 ? 0 : min(kDecKeys, pc.len - key0);
-        const long long pg = max(page, 0);
-        const unsigned char* src = pool + pg * sp + h * sh + (row0_in_page + r_lane) * ss + piece16 * 16;
-        const uint32_t base = ring + slot * C::kSlotBytes;
+        const int n = pc.len - (pc.t * kDecUnit + warp * kDecKeys);
+        if (n <= 0 || page < 0) return;
+        const unsigned char* const src = pool + page * sp + pc.h * sh + (row0_in_page + r_lane) * ss + piece16 * 16;
+        const uint32_t base = dst_lane + slot * C::kSlotBytes;
+        auto dst = [&](int i) {  // row r_lane + i * kRowsAtOnce (r_lane is below kRowsAtOnce, a power of two)
+            return (base ^ ((i * kRowsAtOnce & 7) << 4)) + i * kRowsAtOnce * C::kRowBytes;
+        };
+        if (n >= kDecKeys && ss == C::kRowBytes) {
 #pragma unroll
-        for (int i = 0; i < kDecKeys / kRowsAtOnce; ++i) {
-            const int r = r_lane + i * kRowsAtOnce;
-            cp_async16(base + r * C::kRowBytes + ((piece16 ^ (r & 7)) << 4), src + (r < n ? i * kRowsAtOnce * ss : 0), r < n);
+            for (int i = 0; i < kCopies; ++i) cp_async16(dst(i), src + i * kRowsAtOnce * C::kRowBytes);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const bool take = r_lane + i * kRowsAtOnce < n;
+                cp_async16(dst(i), src + (take ? i * kRowsAtOnce * ss : 0), take);
+            }
         }
         if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
-            if (lane == 0) cp_async16(base + C::kTileBytes, scale + pg * scale_sp + h * scale_sh + row0_in_page, page >= 0);
+            if (lane == 0) cp_async16(smem_u32(scales) + slot * kDecKeys, scale + page * scale_sp + pc.h * scale_sh + row0_in_page);
         }
     };
     auto issue_k = [&](int slot) {
@@ -398,8 +417,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                     my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
                     if (static_cast<unsigned>(my_page) >= static_cast<unsigned>(a.c.n_pages)) {
                         report(a.status, kStatusBadPage);
-                        my_page = -1;
-                        my_row = 0;
+                        my_page = -1;  // (nothing is copied: the keys are whatever the slot held)
                     }
                 }
             }
@@ -441,13 +459,19 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     rows.template prepare<E8>(a, gamma, frag, back);
     __syncthreads();
 
-    // ldmatrix: the row (key) of the slot and the 16-byte piece that this lane names
+    // ldmatrix: the row (key) of the slot and the 16-byte piece that this lane names; piece + 2 j lies 32 j bytes further,
+    // xor-ed below 128 bytes
     const int q8 = lane >> 3;
     const int k_row = (q8 & 1) * 8 + (lane & 7), k_piece = q8 >> 1;
     const int v_row = E8 ? k_row : (q8 >> 1) * 8 + (lane & 7), v_piece = E8 ? k_piece : (q8 & 1);
+    const uint32_t k_lane = ring + k_row * C::kRowBytes + ((k_piece ^ (k_row & 7)) << 4);
+    const uint32_t v_lane = ring + v_row * C::kRowBytes + ((v_piece ^ (v_row & 7)) << 4);
+    auto step32 = [](uint32_t at, int j) { return (at ^ ((j & 3) << 5)) + (j >> 2) * 128; };
     // Probabilities are 2^(score - base + kUp), the base at most kSlack behind the largest score so far: up to 2^15 in f16,
     // whose smallest step is then 2^-35 of the largest probability, up to 2^8 in bf16.
     constexpr bool kHalf = std::is_same<M, __half>::value;
+    // An f16 product of a bf16 call needs no second part: its own is an eighth of what rounding the output to bf16 loses.
+    constexpr bool kSplit = !(E8 && std::is_same<T, __nv_bfloat16>::value);
     constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : 0.f;
 
     int continues = -1, last_cta = 0;
@@ -455,7 +479,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         // ---- one item's part: units cc.t .. cc.t + n - 1
         const int n = min(cc.nt - cc.t, cc.left);
         if (n <= 0) break;
-        const int h = cc.hk / a.row_blocks, row0 = (cc.hk - h * a.row_blocks) * kRows;
+        const int h = cc.h, row0 = (cc.hk - h * a.row_blocks) * kRows;
         DecodeCursor nc = cc;  // the item after this one: its query rows are on their way meanwhile
         nc.t += n;
         nc.left -= n;
@@ -478,21 +502,20 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         }
         // m, mv: bases of the sum and of O (an 8-bit cache's value scales belong to the latter), -inf before the first key
         float o[NT][kDT][4], m[NT][2], mv[NT][2], l[NT][2];
+        float off[NT][2], off_v[NT][2];  // kUp - base, what is added to a score
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
 #pragma unroll
             for (int i = 0; i < kDT; ++i) o[u][i][0] = o[u][i][1] = o[u][i][2] = o[u][i][3] = 0.f;
             m[u][0] = m[u][1] = mv[u][0] = mv[u][1] = -INFINITY;
+            off[u][0] = off[u][1] = off_v[u][0] = off_v[u][1] = 0.f;
             l[u][0] = l[u][1] = 0.f;
         }
         for (int i_unit = 0; i_unit < n; ++i_unit) {
-            const int key0 = (cc.t + i_unit) * kDecUnit + warp * kDecKeys;
-            const bool work = key0 < cc.len;
+            const int keys = cc.len - ((cc.t + i_unit) * kDecUnit + warp * kDecKeys);  // of the sequence, from this step's first on
             arrive(std::false_type{});
             float x[NT][4], w[NT][4];  // scores of keys g (0, 1), g + 8 (2, 3) and heads 2 t4, 2 t4 + 1
-            float ks0 = 1.f, ks1 = 1.f;
-            if (work) {
-                const uint32_t ks = ring + slot * C::kSlotBytes;
+            if (keys > 0) {
                 float s[NT][2][4];  // high and low part of q': two chains of products
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
@@ -503,66 +526,80 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                     for (int u = 0; u < NT; ++u) {
                         const uint4 f = C::kQueryInRegs ? qf[C::kQueryInRegs ? u : 0][C::kQueryInRegs ? j : 0] : frag[(u * kDT + j) * 32 + lane];
                         mma16816<M>(s[u][0], a0, a1, a2, a3, f.x, f.y);
-                        mma16816<M>(s[u][1], a0, a1, a2, a3, f.z, f.w);
+                        if constexpr (kSplit) mma16816<M>(s[u][1], a0, a1, a2, a3, f.z, f.w);
                     }
                 };
-                const uint32_t k_at = ks + k_row * C::kRowBytes;
-                if constexpr (E8) {
+                const uint32_t k_at = k_lane + slot * C::kSlotBytes;
 #pragma unroll
-                    for (int j = 0; j < kDT; j += 2) {
-                        uint32_t r[4];
-                        ldmatrix4(r, k_at + (((j + k_piece) ^ (k_row & 7)) << 4));
+                for (int j = 0; j < kDT; j += E8 ? 2 : 1) {
+                    uint32_t r[4];
+                    ldmatrix4(r, step32(k_at, E8 ? j / 2 : j));
+                    if constexpr (E8) {
 #pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            product(j + y, e4m3_to_half2(r[2 * y]), e4m3_to_half2(r[2 * y + 1]), e4m3_to_half2(r[2 * y] >> 16),
-                                    e4m3_to_half2(r[2 * y + 1] >> 16));
-                    }
-                    const unsigned char* sc = smem + (warp * C::kSlots + slot) * C::kSlotBytes + C::kTileBytes;
-                    ks0 = scale_value(sc[g]);
-                    ks1 = scale_value(sc[g + 8]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < kDT; ++j) {
-                        uint32_t r[4];
-                        ldmatrix4(r, k_at + (((2 * j + k_piece) ^ (k_row & 7)) << 4));
+                        for (int y = 0; y < 2; ++y) {
+                            uint32_t a0, a1, a2, a3;
+                            widen4(r[2 * y], a0, a2);
+                            widen4(r[2 * y + 1], a1, a3);
+                            product(j + y, a0, a1, a2, a3);
+                        }
+                    } else {
                         product(j, r[0], r[1], r[2], r[3]);
                     }
                 }
-                const bool in0 = key0 + g < cc.len, in1 = key0 + g + 8 < cc.len;
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[u][i] = (i < 2 ? in0 : in1) ? (s[u][0][i] + s[u][1][i]) * mul[u][i & 1] * (i < 2 ? ks0 : ks1) : -INFINITY;
-            }
-            leave();
-            arrive(std::true_type{});
-            if (work) {
-                const uint32_t vs = ring + slot * C::kSlotBytes;
-                float ve0 = 0.f, ve1 = 0.f;  // exponents of the value rows
+                float f0 = 1.f, f1 = 1.f;  // scales of the keys
                 if constexpr (E8) {
-                    const unsigned char* sc = smem + (warp * C::kSlots + slot) * C::kSlotBytes + C::kTileBytes;
-                    ve0 = sc[g] == 255 ? NAN : static_cast<float>(sc[g]) - 127.f;
-                    ve1 = sc[g + 8] == 255 ? NAN : static_cast<float>(sc[g + 8]) - 127.f;
+                    f0 = scale_value(scales[slot * kDecKeys + g]);
+                    f1 = scale_value(scales[slot * kDecKeys + g + 8]);
                 }
-                bool above = false;
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        w[u][i] = x[u][i];
-                        above |= x[u][i] > m[u][i & 1] + kSlack;
-                        if constexpr (E8) {
-                            w[u][i] = x[u][i] == -INFINITY ? x[u][i] : x[u][i] + (i < 2 ? ve0 : ve1);
+                        x[u][i] = (kSplit ? s[u][0][i] + s[u][1][i] : s[u][0][i]) * mul[u][i & 1];
+                        if constexpr (E8) x[u][i] *= i < 2 ? f0 : f1;
+                    }
+                if (keys < kDecKeys) {
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (g + 8 * (i >> 1) >= keys) x[u][i] = -INFINITY;
+                }
+            }
+            leave();
+            arrive(std::true_type{});
+            if (keys > 0) {
+                bool above = false;
+                if constexpr (E8) {
+                    const uint32_t e0 = scales[slot * kDecKeys + g], e1 = scales[slot * kDecKeys + g + 8];
+                    const float ve0 = e0 == 255 ? NAN : static_cast<float>(static_cast<int>(e0) - 127);
+                    const float ve1 = e1 == 255 ? NAN : static_cast<float>(static_cast<int>(e1) - 127);
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[u][i] = x[u][i] + (i < 2 ? ve0 : ve1);
                             above |= w[u][i] > mv[u][i & 1] + kSlack;
                         }
+                    if (keys < kDecKeys) {  // (scales behind the sequence are whatever the page holds)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (g + 8 * (i >> 1) >= keys) w[u][i] = -INFINITY;
                     }
-                if (__any_sync(0xffffffffu, above)) {  // move the bases to the maxima so far
-                    auto top = [](float y, float z, float so_far) {
+                }
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) above |= x[u][i] > m[u][i & 1] + kSlack;
+                if (__any_sync(0xffffffffu, above)) {  // move the bases (of the heads whose own scores ask for it) to the maxima
+                    auto top = [](float y, float z, float base) {
                         y = fmaxf(y, z);
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
                         y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-                        return fmaxf(so_far, fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16)));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                        return y > base + kSlack ? y : base;
                     };
 #pragma unroll
                     for (int u = 0; u < NT; ++u)
@@ -579,49 +616,51 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                             }
                             m[u][c] = to;
                             mv[u][c] = to_v;
+                            off[u][c] = to == -INFINITY ? 0.f : kUp - to;
+                            off_v[u][c] = to_v == -INFINITY ? 0.f : kUp - to_v;
                         }
                 }
                 uint32_t pb[NT][4];  // high and low part of the probabilities of keys 0-7, 8-15
 #pragma unroll
                 for (int u = 0; u < NT; ++u) {
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float base = m[u][c] == -INFINITY ? 0.f : m[u][c], base_v = mv[u][c] == -INFINITY ? 0.f : mv[u][c];
-                        const float p0 = ex2(x[u][c] - (base - kUp)), p1 = ex2(x[u][c + 2] - (base - kUp));
-                        l[u][c] += p0 + p1;
-                        w[u][c] = E8 ? ex2(w[u][c] - (base_v - kUp)) : p0;
-                        w[u][c + 2] = E8 ? ex2(w[u][c + 2] - (base_v - kUp)) : p1;
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = ex2(x[u][i] + off[u][i & 1]);
+                        l[u][i & 1] += p;
+                        w[u][i] = E8 ? ex2(w[u][i] + off_v[u][i & 1]) : p;
                     }
-                    split2_probabilities<M, !E8>(w[u][0], w[u][1], pb[u][0], pb[u][2]);
-                    split2_probabilities<M, !E8>(w[u][2], w[u][3], pb[u][1], pb[u][3]);
+                    if constexpr (kSplit) {
+                        split2_probabilities<M, !E8>(w[u][0], w[u][1], pb[u][0], pb[u][2]);
+                        split2_probabilities<M, !E8>(w[u][2], w[u][3], pb[u][1], pb[u][3]);
+                    } else {
+                        pb[u][0] = Num<M>::pack(w[u][0], w[u][1]);
+                        pb[u][1] = Num<M>::pack(w[u][2], w[u][3]);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) pb[u][i] = transpose8x8(pb[u][i]);
+                    for (int i = 0; i < (kSplit ? 4 : 2); ++i) pb[u][i] = transpose8x8(pb[u][i]);
                 }
                 auto product = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u) {
                         mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][0], pb[u][1]);
-                        mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][2], pb[u][3]);
+                        if constexpr (kSplit) mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][2], pb[u][3]);
                     }
                 };
-                const uint32_t v_at = vs + v_row * C::kRowBytes;
-                if constexpr (E8) {
+                const uint32_t v_at = v_lane + slot * C::kSlotBytes;
 #pragma unroll
-                    for (int i = 0; i < kDT; i += 2) {
-                        uint32_t r[4];
-                        ldmatrix4_trans(r, v_at + (((i + v_piece) ^ (v_row & 7)) << 4));
+                for (int i = 0; i < kDT; i += E8 ? 2 : 1) {
+                    uint32_t r[4];
+                    ldmatrix4_trans(r, step32(v_at, E8 ? i / 2 : i));
+                    if constexpr (E8) {
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             // bytes {key 2t col 2g, key 2t col 2g+1, key 2t+1 col 2g, key 2t+1 col 2g+1}
-                            const uint32_t y0 = __byte_perm(r[2 * y], 0, 0x3120), y1 = __byte_perm(r[2 * y + 1], 0, 0x3120);
-                            product(i + y, e4m3_to_half2(y0), e4m3_to_half2(y0 >> 16), e4m3_to_half2(y1), e4m3_to_half2(y1 >> 16));
+                            uint32_t a0, a1, a2, a3;
+                            widen4(__byte_perm(r[2 * y], 0, 0x3120), a0, a1);
+                            widen4(__byte_perm(r[2 * y + 1], 0, 0x3120), a2, a3);
+                            product(i + y, a0, a1, a2, a3);
                         }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kDT; ++i) {
-                        uint32_t r[4];
-                        ldmatrix4_trans(r, v_at + (((2 * i + v_piece) ^ (v_row & 7)) << 4));
+                    } else {
                         product(i, r[0], r[1], r[2], r[3]);
                     }
                 }
