@@ -9,7 +9,9 @@
 // Work split.  The unit of work is 64 keys of one (sequence, KV head).  All units of the launch are laid in one line and
 // every CTA takes an equal piece of it, found from the lengths on the device: ragged batches and single long sequences
 // load all SMs alike, and a captured launch follows its lengths.  A CTA's piece covers whole (sequence, head) items and
-// at most two broken ones; a broken item's pieces meet in the workspace and are joined by decode_join_kernel.
+// at most two broken ones; a broken item's parts meet in the workspace, where the CTA that comes last joins them, in the
+// order of the line whoever that is: 16 at a time, and if there are more, the joined sixteens once more.  (A second kernel
+// for it cost 2 us of a call, and its serial pass over 37 parts of a long sequence 12 us.)
 //
 // Inside a CTA each of the four warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
 // into its own ring of slots in shared memory (cp.async, across item borders), and keeps its own sum and output; the four
@@ -39,6 +41,7 @@ struct DecodeArgs {
     long long q_sb, q_sh, o_sb, o_sh;   // element strides
     const int* lengths;
     float* ws;                          // decode_workspace_floats() floats
+    unsigned int* arrived;              // a word per CTA, zero before and after the launch (see join_words)
     int B, Hkv, G, row_blocks;          // G query heads per KV head in row_blocks blocks
     int n_pos;
     float eps, scale_log2e;
@@ -267,14 +270,105 @@ template <int D, typename T, int NT> struct QueryRows {
     }
 };
 
-// Where the broken items' parts and what joins them lie in the workspace: for each CTA two parts (0: an item that began
-// in an earlier CTA, 1: one that begins here), then for each CTA {item that begins here and goes on, or -1; last CTA of it}.
+// Where the broken items' parts lie in the workspace: for each CTA two (0: of an item that began in an earlier CTA, 1: of
+// one that begins here).  Behind them are words for `arrived`, for launches that have none of the library's.
 template <int D, bool E8, int NT> __host__ __device__ constexpr long long decode_part_at(int cta, int which) {
     return (2LL * cta + which) * DecodeCfg<D, E8, NT>::kPartFloats;
 }
 template <int D, bool E8, int NT> __host__ __device__ constexpr long long decode_workspace_floats(int ctas) {
-    return decode_part_at<D, E8, NT>(ctas, 0) + 4LL * ctas;
+    return decode_part_at<D, E8, NT>(ctas, 0) + ctas;
 }
+
+// Joining.  Item parts of CTAs first .. last (one that begins in `first`); groups of kJoin consecutive ones.  A CTA's word
+// counts in three fields: parts that have arrived of the group whose first part is its part 0 (bits 0-7) or its part 1
+// (8-15), and joined groups of the item that begins in it (16-31).  Who completes a field takes it back to zero.
+constexpr int kJoin = 16;
+
+template <int D, typename T, bool E8, int NT> struct DecodeJoin {
+    using C = DecodeCfg<D, E8, NT>;
+    static constexpr int kRows = C::kRows;
+    const DecodeArgs& a;
+    float* scratch;  // shared memory: maxima and sums of the parts, and of the result
+    int* s_flag;
+
+    // All threads: count one more in the field; true for the CTA that completes `count`.
+    __device__ __forceinline__ bool arrive(int cta, int shift, int count) const {
+        __threadfence();  // the part is visible before it counts
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const unsigned int before = atomicAdd(a.arrived + cta, 1u << shift);
+            const bool all = static_cast<int>(before >> shift & (shift == 16 ? 0xffffu : 0xffu)) == count - 1;
+            if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
+            __threadfence();
+            *s_flag = all;
+        }
+        __syncthreads();
+        return *s_flag != 0;
+    }
+    // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.
+    __device__ __forceinline__ void sum(int first, int from, int stride, int n, float* out, int b, int h, int row0) const {
+        float* const top = scratch;
+        float* const total = top + kRows;
+        float* const m = total + kRows;  // [n][kRows]
+        float* const l = m + n * kRows;
+        auto part = [&](int i) { return a.ws + decode_part_at<D, E8, NT>(from + i * stride, from + i * stride == first); };
+        for (int i = threadIdx.x; i < n * kRows; i += kDecThreads) {
+            m[i] = __ldcg(part(i / kRows) + kRows * D + i % kRows);
+            l[i] = __ldcg(part(i / kRows) + kRows * D + kRows + i % kRows);
+        }
+        __syncthreads();
+        if (threadIdx.x < kRows) {
+            const int r = threadIdx.x;
+            float t = -INFINITY, s = 0.f;
+            for (int i = 0; i < n; ++i) t = fmaxf(t, m[i * kRows + r]);
+            for (int i = 0; i < n; ++i) {
+                const float f = m[i * kRows + r] == -INFINITY ? 0.f : exp2f(m[i * kRows + r] - t);
+                s += l[i * kRows + r] * f;
+                m[i * kRows + r] = f;
+            }
+            top[r] = t;
+            total[r] = s;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < kRows * (D / 4); e += kDecThreads) {
+            const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+            if (row0 + r >= a.G) break;  // (rows go up with e)
+            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(part(i) + r * D + d));
+                const float f = m[i * kRows + r];
+                z.x += x.x * f;
+                z.y += x.y * f;
+                z.z += x.z * f;
+                z.w += x.w * f;
+            }
+            if (out != nullptr) {
+                *reinterpret_cast<float4*>(out + r * D + d) = z;
+                if (d == 0) {
+                    out[kRows * D + r] = top[r];
+                    out[kRows * D + kRows + r] = total[r];
+                }
+            } else {
+                T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
+                const float inv = 1.f / total[r];
+                *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+            }
+        }
+        __syncthreads();
+    }
+    // This CTA's part of the item is in its place (`dead`: it never will be; only the counts have to go on).
+    __device__ __forceinline__ void part_done(int first, int last, int b, int hk, int h, bool dead) const {
+        const int cta = blockIdx.x, row0 = (hk - h * a.row_blocks) * kRows;
+        const int groups = (last - first) / kJoin + 1, from = first + (cta - first) / kJoin * kJoin;
+        const int n = min(kJoin, last - from + 1);
+        if (n > 1 && !arrive(from, from == first ? 8 : 0, n)) return;
+        float* const place = groups == 1 ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == first);
+        if (n > 1 && !dead) sum(first, from, 1, n, place, b, h, row0);
+        if (groups == 1 || !arrive(first, 16, groups) || dead) return;
+        sum(first, first, kJoin, groups, nullptr, b, h, row0);
+    }
+};
 
 template <int D, typename T, bool E8, int NT>
 __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm) decode_kernel(const DecodeArgs a) {
@@ -282,10 +376,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     using M = typename std::conditional<E8, __half, T>::type;  // type of the products' operands
     constexpr int kDT = D / 16, kRows = C::kRows;
     __shared__ long long s_sum[kDecWarps], s_first;
-    __shared__ int s_b, s_dead;
+    __shared__ int s_b, s_dead, s_flag;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int HK = a.Hkv * a.row_blocks, n_ctas = gridDim.x;
-    int* const meta = reinterpret_cast<int*>(a.ws + decode_part_at<D, E8, NT>(n_ctas, 0));
     if (tid == 0) s_dead = *reinterpret_cast<volatile int*>(a.status);  // (one reading for the whole CTA)
 
     // ---- this CTA's piece of the line of units
@@ -305,7 +398,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     }
     if (lane == 31) s_sum[warp] = before;
     __syncthreads();
-    if (s_dead != 0) return;
+    const bool dead = s_dead != 0;  // then nothing is read or written but the counts of the joins, which other CTAs may wait for
     long long total = 0;
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
@@ -330,17 +423,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         s_first = at;
     }
     // sequences without rows have no units: their output is zero
-    for (int b = blockIdx.x; b < a.B; b += n_ctas)
+    for (int b = blockIdx.x; b < a.B && !dead; b += n_ctas)
         if (cached_rows(a, b) == 0) {
             const int Hq = a.Hkv * a.G;
             for (int i = tid; i < Hq * (D / 8); i += kDecThreads)
                 reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
                     make_uint4(0, 0, 0, 0);
         }
-    if (u0 >= total) {
-        if (tid == 0) meta[2 * blockIdx.x] = -1;
-        return;
-    }
+    if (u0 >= total) return;
     __syncthreads();
     DecodeCursor cc;
     cc.b = s_b;
@@ -353,6 +443,36 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         cc.h = cc.hk / a.row_blocks;
     }
     cc.left = static_cast<int>(u1 - u0);
+    // the broken items: the one that began before this piece or fills it, and the one that begins in it and goes on
+    int first0 = -1, last0 = 0, b0 = 0, hk0 = 0, h0 = 0, last1 = -1, b1 = 0, hk1 = 0, h1 = 0;
+    if (cc.t > 0) {
+        first0 = static_cast<int>((u0 - cc.t) / piece);
+        last0 = static_cast<int>((u0 - cc.t + cc.nt - 1) / piece);
+        b0 = cc.b;
+        hk0 = cc.hk;
+        h0 = cc.h;
+    }
+    auto begins_and_goes_on = [&](int n) {  // n units of item cc here
+        if (cc.t > 0 || n == cc.nt) return;
+        last1 = static_cast<int>((u1 - 1 + (cc.nt - n)) / piece);
+        b1 = cc.b;
+        hk1 = cc.hk;
+        h1 = cc.h;
+    };
+    if (dead) {
+        while (cc.left > 0) {
+            const int n = min(cc.nt - cc.t, cc.left);
+            if (n <= 0) break;
+            begins_and_goes_on(n);
+            cc.t += n;
+            cc.left -= n;
+            if (cc.left > 0) cc.next_item(a, HK);
+        }
+        const DecodeJoin<D, T, E8, NT> join{a, nullptr, &s_flag};
+        if (first0 >= 0) join.part_done(first0, last0, b0, hk0, h0, true);
+        if (last1 >= 0) join.part_done(blockIdx.x, last1, b1, hk1, h1, true);
+        return;
+    }
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
     // eight rows of a column block lie in different banks)
@@ -474,7 +594,6 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     constexpr bool kSplit = !(E8 && std::is_same<T, __nv_bfloat16>::value);
     constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : 0.f;
 
-    int continues = -1, last_cta = 0;
     while (cc.left > 0) {
         // ---- one item's part: units cc.t .. cc.t + n - 1
         const int n = min(cc.nt - cc.t, cc.left);
@@ -700,10 +819,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 }
             }
         const bool whole = n == cc.nt;
-        if (!whole && cc.t == 0) {  // begins here and goes on: to its last unit
-            continues = cc.b * HK + cc.hk;
-            last_cta = static_cast<int>((u1 - 1 + (cc.nt - n)) / piece);
-        }
+        begins_and_goes_on(n);
         float* const part = a.ws + decode_part_at<D, E8, NT>(blockIdx.x, cc.t == 0 ? 1 : 0);
         float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
         // eight rows and 128 columns at a time: warps 2 and 3 leave theirs, 0 and 1 add theirs, all add the two copies
@@ -754,43 +870,10 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         cc = nc;
     }
     cp_async_wait<0>();
-    if (tid == 0) {
-        meta[2 * blockIdx.x] = continues;
-        meta[2 * blockIdx.x + 1] = last_cta;
-    }
-}
-
-// Joins the broken items: CTA i the one that begins in CTA i of decode_kernel, in the order of the parts.
-template <int D, typename T, bool E8, int NT>
-__global__ void __launch_bounds__(kDecThreads) decode_join_kernel(const DecodeArgs a) {
-    using C = DecodeCfg<D, E8, NT>;
-    constexpr int kRows = C::kRows;
-    const int n_ctas = gridDim.x, HK = a.Hkv * a.row_blocks, first = blockIdx.x;
-    if (*reinterpret_cast<volatile int*>(a.status) != 0) return;
-    const int* const meta = reinterpret_cast<const int*>(a.ws + decode_part_at<D, E8, NT>(n_ctas, 0));
-    const int item = meta[2 * first], last = meta[2 * first + 1];
-    if (item < 0) return;
-    const int b = item / HK, hk = item - b * HK, h = hk / a.row_blocks, row0 = (hk - h * a.row_blocks) * kRows;
-    for (int i = threadIdx.x; i < kRows * (D / 4); i += kDecThreads) {
-        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-        if (row0 + r >= a.G) break;
-        float top = -INFINITY, sum = 0.f;
-        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = first; c <= last; ++c) top = fmaxf(top, a.ws[decode_part_at<D, E8, NT>(c, c == first) + kRows * D + r]);
-        for (int c = first; c <= last; ++c) {
-            const float* part = a.ws + decode_part_at<D, E8, NT>(c, c == first);
-            const float m = part[kRows * D + r], f = m == -INFINITY ? 0.f : exp2f(m - top);
-            const float4 x = *reinterpret_cast<const float4*>(part + r * D + d);
-            sum += part[kRows * D + kRows + r] * f;
-            z.x += x.x * f;
-            z.y += x.y * f;
-            z.z += x.z * f;
-            z.w += x.w * f;
-        }
-        T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
-        const float inv = 1.f / sum;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
-    }
+    __syncthreads();  // (the ring serves the joins)
+    const DecodeJoin<D, T, E8, NT> join{a, reinterpret_cast<float*>(smem), &s_flag};
+    if (first0 >= 0) join.part_done(first0, last0, b0, hk0, h0, false);
+    if (last1 >= 0) join.part_done(blockIdx.x, last1, b1, hk1, h1, false);
 }
 
 }  // namespace kf

@@ -137,5 +137,58 @@ inline int sm_count() {
     return cached[dev];
 }
 
+// Slots of a table in device memory that captured launches own: a captured launch runs again with every replay of its
+// graph, next to whatever else is running, so it gets a slot for itself, which the graph, its clones and its executable
+// forms own together and give back when the last of them is destroyed.  (Plain data: graphs may outlive static objects.)
+template <int N> struct GraphSlots {
+    std::atomic_flag busy = ATOMIC_FLAG_INIT;
+    int back[N], n_back, n_taken;  // slots given back; slots taken at least once
+    int take() {                   // -1: none left
+        while (busy.test_and_set(std::memory_order_acquire)) {}
+        const int s = n_back > 0 ? back[--n_back] : n_taken < N ? n_taken++ : -1;
+        busy.clear(std::memory_order_release);
+        return s;
+    }
+    void give_back(int slot) {
+        while (busy.test_and_set(std::memory_order_acquire)) {}
+        back[n_back++] = slot;
+        busy.clear(std::memory_order_release);
+    }
+};
+
+// The slot of the launch about to be made into `st`: one of the first `eager` in turn (two launches could only share one if
+// one were still running when that many later ones have been started), or, while the stream is being captured, one of SLOTS
+// behind them; -1 when every one of those is taken.
+template <auto& SLOTS> int launch_slot(cudaStream_t st, std::atomic<unsigned int>& turn, int eager, int* out) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo_v2(st, &capture, nullptr, &graph, nullptr, nullptr) != cudaSuccess) {
+        cudaGetLastError();  // (the legacy stream next to a capture elsewhere: the launch itself reports that)
+        capture = cudaStreamCaptureStatusNone;
+    }
+    if (capture != cudaStreamCaptureStatusActive) {
+        *out = static_cast<int>(turn.fetch_add(1, std::memory_order_relaxed) % static_cast<unsigned int>(eager));
+        return KF_OK;
+    }
+    *out = -1;
+    const int slot = SLOTS.take();
+    if (slot < 0) return KF_OK;
+    cudaUserObject_t owner = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&owner, reinterpret_cast<void*>(static_cast<intptr_t>(slot)),
+                                         [](void* tag) { SLOTS.give_back(static_cast<int>(reinterpret_cast<intptr_t>(tag))); }, 1,
+                                         cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        SLOTS.give_back(slot);
+        return fail(KF_ECUDA, "cudaUserObjectCreate failed: %s", cudaGetErrorString(e));
+    }
+    e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        cudaUserObjectRelease(owner, 1);  // (gives the slot back)
+        return fail(KF_ECUDA, "cudaGraphRetainUserObject failed: %s", cudaGetErrorString(e));
+    }
+    *out = eager + slot;
+    return KF_OK;
+}
+
 }  // namespace host
 }  // namespace kf

@@ -215,20 +215,7 @@ constexpr int kAutoPersistMinS = 2048, kAutoPersistMaxS = 8192;
 constexpr int kSchedSlots = 1024, kGraphSlots = 1 << 14;
 __device__ unsigned int g_sched[kSchedSlots + kGraphSlots][2];
 
-std::atomic_flag g_slots_busy = ATOMIC_FLAG_INIT;  // guards the three below (plain data: graphs may outlive static objects)
-int g_slots_back[kGraphSlots], g_n_back, g_n_taken;  // slots given back; slots taken at least once
-
-int take_graph_slot() {  // -1: none left
-    while (g_slots_busy.test_and_set(std::memory_order_acquire)) {}
-    const int s = g_n_back > 0 ? g_slots_back[--g_n_back] : g_n_taken < kGraphSlots ? g_n_taken++ : -1;
-    g_slots_busy.clear(std::memory_order_release);
-    return s;
-}
-void CUDART_CB give_back_graph_slot(void* slot) {
-    while (g_slots_busy.test_and_set(std::memory_order_acquire)) {}
-    g_slots_back[g_n_back++] = static_cast<int>(reinterpret_cast<intptr_t>(slot));
-    g_slots_busy.clear(std::memory_order_release);
-}
+GraphSlots<kGraphSlots> g_sched_graph_slots;
 
 // The counters of the launch about to be made into `st`; NULL: it is being captured and every graph slot is taken.
 int sched_slot(cudaStream_t st, unsigned int** out) {
@@ -237,33 +224,9 @@ int sched_slot(cudaStream_t st, unsigned int** out) {
     void* p = nullptr;
     cudaError_t e = symbol_address(cache, g_sched, &p);
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(work counters) failed: %s", cudaGetErrorString(e));
-    unsigned int* const bp = static_cast<unsigned int*>(p);
-    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-    cudaGraph_t graph = nullptr;
-    if (cudaStreamGetCaptureInfo_v2(st, &capture, nullptr, &graph, nullptr, nullptr) != cudaSuccess) {
-        cudaGetLastError();  // (the legacy stream next to a capture elsewhere: the launch itself reports that)
-        capture = cudaStreamCaptureStatusNone;
-    }
-    if (capture != cudaStreamCaptureStatusActive) {
-        *out = bp + 2 * (turn.fetch_add(1, std::memory_order_relaxed) % kSchedSlots);
-        return KF_OK;
-    }
-    *out = nullptr;
-    const int slot = take_graph_slot();
-    if (slot < 0) return KF_OK;
-    cudaUserObject_t owner = nullptr;
-    void* const tag = reinterpret_cast<void*>(static_cast<intptr_t>(slot));
-    e = cudaUserObjectCreate(&owner, tag, give_back_graph_slot, 1, cudaUserObjectNoDestructorSync);
-    if (e != cudaSuccess) {
-        give_back_graph_slot(tag);
-        return fail(KF_ECUDA, "cudaUserObjectCreate failed: %s", cudaGetErrorString(e));
-    }
-    e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
-    if (e != cudaSuccess) {
-        cudaUserObjectRelease(owner, 1);  // (gives the slot back)
-        return fail(KF_ECUDA, "cudaGraphRetainUserObject failed: %s", cudaGetErrorString(e));
-    }
-    *out = bp + 2 * (kSchedSlots + slot);
+    int slot = -1;
+    if (int r = launch_slot<g_sched_graph_slots>(st, turn, kSchedSlots, &slot)) return r;
+    *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + 2 * slot;
     return KF_OK;
 }
 

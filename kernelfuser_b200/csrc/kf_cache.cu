@@ -106,7 +106,30 @@ template <int D, typename T, bool E8> int launch_read(const kf::ReadArgs& a, cud
                                                dim3(kf::kRowsThreads), 0, st, a));
 }
 
-template <int D, bool E8, int NT> int decode_ctas() { return sm_count() * kf::DecodeCfg<D, E8, NT>::kCtasPerSm; }
+// Words in which the CTAs of a decode launch count what has arrived for a join: a row of them per launch, zero between
+// launches (in the library image; the CTA that completes a count takes it back).  Launches into a stream take the first
+// kJoinSlots rows in turn, a captured one has one of its own.
+constexpr int kMaxCtas = 512, kJoinSlots = 1024, kJoinGraphSlots = 4096;
+__device__ unsigned int g_arrived[kJoinSlots + kJoinGraphSlots][kMaxCtas];
+GraphSlots<kJoinGraphSlots> g_join_graph_slots;
+
+// NULL: the launch is being captured and every graph slot is taken.
+int join_words(cudaStream_t st, unsigned int** out) {
+    static SymbolCache cache;
+    static std::atomic<unsigned int> turn{0};
+    void* p = nullptr;
+    cudaError_t e = symbol_address(cache, g_arrived, &p);
+    if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(join words) failed: %s", cudaGetErrorString(e));
+    int slot = -1;
+    if (int r = launch_slot<g_join_graph_slots>(st, turn, kJoinSlots, &slot)) return r;
+    *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + static_cast<size_t>(slot) * kMaxCtas;
+    return KF_OK;
+}
+
+template <int D, bool E8, int NT> int decode_ctas() {
+    const int n = sm_count() * kf::DecodeCfg<D, E8, NT>::kCtasPerSm;
+    return n < kMaxCtas ? n : kMaxCtas;
+}
 
 template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::DecodeArgs& a, cudaStream_t st) {
     constexpr auto kern = kf::decode_kernel<D, T, E8, NT>;
@@ -120,8 +143,15 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
                            ((a.c.capacity + kf::kDecUnit - 1) / kf::kDecUnit);
     const long long want = (most + kf::kDecMinUnits - 1) / kf::kDecMinUnits, fit = decode_ctas<D, E8, NT>();
     const unsigned grid = (unsigned)(want < fit ? want : fit);
-    if (int r = launched("decode_attention", launch_kernel(kern, dim3(grid), dim3(kf::kDecThreads), smem, st, args))) return r;
-    return launched("decode_attention", launch_kernel(kf::decode_join_kernel<D, T, E8, NT>, dim3(grid), dim3(kf::kDecThreads), 0, st, args));
+    if (grid > 1) {
+        if (int r = join_words(st, &args.arrived)) return r;
+        if (args.arrived == nullptr) {  // then words in the workspace, cleared by the graph itself
+            args.arrived = reinterpret_cast<unsigned int*>(a.ws + kf::decode_part_at<D, E8, NT>((int)fit, 0));
+            e = cudaMemsetAsync(args.arrived, 0, sizeof(unsigned int) * grid, st);
+            if (e != cudaSuccess) return fail(KF_ECUDA, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
+        }
+    }
+    return launched("decode_attention", launch_kernel(kern, dim3(grid), dim3(kf::kDecThreads), smem, st, args));
 }
 
 template <int D, typename T, bool E8> int launch_decode(const kf::DecodeArgs& a, cudaStream_t st) {

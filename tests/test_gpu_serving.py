@@ -102,6 +102,49 @@ def test_long_sequences_are_split_and_joined(cache, lengths, hq, hkv, d):
         assert torch.equal(kf.decode_attention(q, p.cache, p.pages, ints(lengths), gq, cos, sin), got)
 
 
+def test_more_captured_launches_than_join_words():
+    # a captured launch has words of its own to count in, 4096 at a time; a further one gets them from its workspace
+    lengths, most = [3000, 70], 4300
+    p = Paged(lengths, 1, 128, 64, BF, seed=50)
+    q, n = rand(51, 2, 4, 1, 128), ints(lengths)
+    want = kf.decode_attention(q, p.cache, p.pages, n)
+    out = torch.empty_like(want)
+    ws = torch.empty(kf.decode_workspace_bytes(q, p.cache), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(most):
+                kf.decode_attention(q, p.cache, p.pages, n, out=out, workspace=ws)
+        out.zero_()
+        for _ in range(2):
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        g.reset()
+        del g
+    done()
+
+
+def test_joins_after_a_status():
+    # CTAs that find the status word set still count, so that the words are clear for the next launch
+    lengths = [40000, 9000]
+    p = Paged(lengths, 1, 128, 64, BF, seed=52)
+    q, n = rand(53, 2, 4, 1, 128), ints(lengths)
+    want = kf.decode_attention(q, p.cache, p.pages, n)
+    done()
+    for _ in range(1100):  # every row of words in turn
+        bad = p.pages.clone() if _ == 0 else bad
+        if _ == 0:
+            bad[0, 3] = -1
+        kf.decode_attention(q, p.cache, bad, n)
+    with pytest.raises(kf.KernelStatusError, match="911"):
+        kf.check_status()
+    for _ in range(1100):
+        got = kf.decode_attention(q, p.cache, p.pages, n)
+    done()
+    assert torch.equal(got, want)
+
+
 def test_many_sequences():
     # more sequences than threads of a CTA, runs of empty ones among them
     lengths = [(37 * b) % 150 if b % 7 and not 200 < b < 420 else 0 for b in range(700)]
