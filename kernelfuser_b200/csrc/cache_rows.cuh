@@ -55,12 +55,129 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return __uint_as_float(byte == 255 ? 0x7fffffffu : byte == 0 ? 0x00400000u : byte << 23);
 }
 
+// A row of D values over LPR lanes: lane i holds columns W i .. W i + W - 1 and their rotation partners D/2 further.  The
+// arithmetic (order of the sum of squares included) does not depend on LPR: a row gets the same bits wherever it is done.
+template <int D, int LPR> struct Row {
+    static constexpr int W = D / 2 / LPR, kWords = W / 2;
+    using Words = uint32_t[2][kWords];  // packed 16-bit values of both halves
+    float x[2][W];
+
+    template <bool STREAM> __device__ static __forceinline__ void load(Words& w, const void* row, int lane) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const char* const p = static_cast<const char*>(row) + half * D + lane * (2 * W);  // (bytes)
+            if constexpr (kWords == 4) {
+                const uint4 v = STREAM ? __ldcs(reinterpret_cast<const uint4*>(p)) : __ldg(reinterpret_cast<const uint4*>(p));
+                w[half][0] = v.x;
+                w[half][1] = v.y;
+                w[half][2] = v.z;
+                w[half][3] = v.w;
+            } else if constexpr (kWords == 2) {
+                const uint2 v = STREAM ? __ldcs(reinterpret_cast<const uint2*>(p)) : __ldg(reinterpret_cast<const uint2*>(p));
+                w[half][0] = v.x;
+                w[half][1] = v.y;
+            } else {
+                w[half][0] = STREAM ? __ldcs(reinterpret_cast<const uint32_t*>(p)) : __ldg(reinterpret_cast<const uint32_t*>(p));
+            }
+        }
+    }
+    template <typename T> __device__ __forceinline__ void unpack(const Words& w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const float2 v = Num<T>::unpack(w[half][i]);
+                x[half][2 * i] = v.x;
+                x[half][2 * i + 1] = v.y;
+            }
+    }
+    template <typename T> __device__ __forceinline__ void norm(const Words& gamma, float eps) {
+        constexpr int kUnit = D / 64, kUnits = W / kUnit;  // a thirty-second of the row at a time
+        float ss[kUnits];
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            ss[u] = 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int i = 0; i < kUnit; ++i) ss[u] = fmaf(x[half][u * kUnit + i], x[half][u * kUnit + i], ss[u]);
+        }
+#pragma unroll
+        for (int m = 1; m < kUnits; m *= 2)
+#pragma unroll
+            for (int u = 0; u < kUnits; u += 2 * m) ss[u] += ss[u + m];
+#pragma unroll
+        for (int m = 1; m < LPR; m *= 2) ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], m);
+        const float inv = rsqrtf(fmaf(ss[0], 1.0f / static_cast<float>(D), eps));
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const float2 g = Num<T>::unpack(gamma[half][i]);
+                x[half][2 * i] = __fmul_rn(__fmul_rn(x[half][2 * i], inv), g.x);
+                x[half][2 * i + 1] = __fmul_rn(__fmul_rn(x[half][2 * i + 1], inv), g.y);
+            }
+    }
+    template <typename T> __device__ __forceinline__ void rotate(const Words& c, const Words& s) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const float2 cl = Num<T>::unpack(c[0][i]), ch = Num<T>::unpack(c[1][i]);
+            const float2 sl = Num<T>::unpack(s[0][i]), sh = Num<T>::unpack(s[1][i]);
+            const float lo0 = x[0][2 * i], lo1 = x[0][2 * i + 1], hi0 = x[1][2 * i], hi1 = x[1][2 * i + 1];
+            x[0][2 * i] = fmaf(lo0, cl.x, -__fmul_rn(hi0, sl.x));
+            x[0][2 * i + 1] = fmaf(lo1, cl.y, -__fmul_rn(hi1, sl.y));
+            x[1][2 * i] = fmaf(hi0, ch.x, __fmul_rn(lo0, sh.x));
+            x[1][2 * i + 1] = fmaf(hi1, ch.y, __fmul_rn(lo1, sh.y));
+        }
+    }
+    // bits of the largest magnitude of the row (a NaN is the largest)
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < W; ++i) m = max(m, __float_as_uint(x[half][i]) & 0x7fffffffu);
+#pragma unroll
+        for (int d = 1; d < LPR; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
+    }
+    // The row in the cache's type: `put(byte offset, value)` with a value of 2, 4, 8 or 16 bytes.  Returns the scale's byte.
+    template <typename T, bool E8, typename F> __device__ __forceinline__ uint32_t store(int lane, F&& put) const {
+        uint32_t e = 0;
+        if constexpr (E8) {
+            e = scale_byte(largest());
+            const float f = e == 255 ? 1.f : __uint_as_float((254u - e) << 23);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[(W + 3) / 4] = {};
+#pragma unroll
+                for (int i = 0; i < W; i += 2) w[i / 4] |= pack_e4m3(x[half][i] * f, x[half][i + 1] * f) << (8 * (i % 4));
+                const int at = half * (D / 2) + lane * W;
+                if constexpr (W == 8) put(at, make_uint2(w[0], w[1]));
+                else if constexpr (W == 4) put(at, w[0]);
+                else put(at, static_cast<uint16_t>(w[0]));
+            }
+        } else {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t w[kWords];
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) w[i] = Num<T>::pack(x[half][2 * i], x[half][2 * i + 1]);
+                const int at = half * D + lane * (2 * W);
+                if constexpr (kWords == 4) put(at, make_uint4(w[0], w[1], w[2], w[3]));
+                else if constexpr (kWords == 2) put(at, make_uint2(w[0], w[1]));
+                else put(at, w[0]);
+            }
+        }
+        return e;
+    }
+};
+
 struct AppendArgs {
     CacheView c;
     const void *k, *v, *gamma, *cos, *sin;       // gamma, tables: may be null
     long long k_sb, k_sh, k_ss, v_sb, v_sh, v_ss;  // element strides
     const int *start, *counts;                   // counts may be null: all S rows
-    int newest;                                  // one row per sequence, at start[b] - 1 where start[b] > 0
     int B, H, S, n_pos, heads_per_group;
     float eps;
     int* status;
@@ -68,8 +185,8 @@ struct AppendArgs {
 
 constexpr int kRowsThreads = 256;
 
-// A row's lane owns columns [8i, 8i+8) and their rotation partners, as in the row-prepare kernel; a group of D/16 lanes
-// walks over heads of one position, so that the tables are read once for them.
+// A group of D/16 lanes walks over heads of one position, so that the tables are read once for them; a lane's columns are
+// two 16-byte pieces of a row.
 template <int D, typename T, bool E8>
 __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendArgs a) {
     constexpr int LPR = D / 16;
@@ -81,8 +198,7 @@ __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendA
     int pos = 0, page = 0, row = 0;
     if (valid) {
         if (a.counts != nullptr) valid = s < a.counts[b];
-        long long p = static_cast<long long>(a.start[b]) + s;
-        if (a.newest) valid = --p >= 0;
+        const long long p = static_cast<long long>(a.start[b]) + s;
         if (valid && (p < 0 || p >= a.c.capacity)) {
             report(a.status, kStatusBadLength);
             valid = false;
@@ -101,105 +217,39 @@ __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendA
             }
         }
     }
-    const bool rope = a.cos != nullptr;
-    uint4 glo = make_uint4(0, 0, 0, 0), ghi = glo, clo = glo, chi = glo, slo = glo, shi = glo;
-    if (a.gamma != nullptr) {
-        const uint4* g4 = reinterpret_cast<const uint4*>(a.gamma);
-        glo = __ldg(g4 + sub);
-        ghi = __ldg(g4 + LPR + sub);
-    }
-    if (rope && valid) {
-        const uint4* c4 = reinterpret_cast<const uint4*>(a.cos) + static_cast<long long>(pos) * (D / 8);
-        const uint4* s4 = reinterpret_cast<const uint4*>(a.sin) + static_cast<long long>(pos) * (D / 8);
-        clo = __ldg(c4 + sub);
-        chi = __ldg(c4 + LPR + sub);
-        slo = __ldg(s4 + sub);
-        shi = __ldg(s4 + LPR + sub);
+    using R = Row<D, LPR>;
+    typename R::Words gamma, cos, sin;
+    if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, sub);
+    if (a.cos != nullptr) {
+        R::template load<false>(cos, reinterpret_cast<const T*>(a.cos) + static_cast<long long>(valid ? pos : 0) * D, sub);
+        R::template load<false>(sin, reinterpret_cast<const T*>(a.sin) + static_cast<long long>(valid ? pos : 0) * D, sub);
     }
     const int h0 = blockIdx.y * a.heads_per_group, h1 = min(h0 + a.heads_per_group, a.H);
     const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + s * a.k_ss;
     const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + s * a.v_ss;
     unsigned char* kd = a.c.k + page * a.c.k_sp + row * a.c.k_ss;
     unsigned char* vd = a.c.v + page * a.c.v_sp + row * a.c.v_ss;
-
-    // one row of 16 floats a lane to the cache
-    auto put = [&](const float (&x)[16], unsigned char* dst, unsigned char* scale) {
-        if constexpr (E8) {
-            uint32_t amax = 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);  // (a NaN is the largest)
-#pragma unroll
-            for (int m = LPR / 2; m >= 1; m >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-            const uint32_t e = scale_byte(amax);
-            const float f = e == 255 ? 1.f : __uint_as_float((254u - e) << 23);
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[i] = pack_e4m3(x[4 * i] * f, x[4 * i + 1] * f) | (pack_e4m3(x[4 * i + 2] * f, x[4 * i + 3] * f) << 16);
-            if (valid) {
-                reinterpret_cast<uint2*>(dst)[sub] = make_uint2(w[0], w[1]);
-                reinterpret_cast<uint2*>(dst)[LPR + sub] = make_uint2(w[2], w[3]);
-                if (sub == 0) *scale = static_cast<unsigned char>(e);
-            }
-        } else if (valid) {
-            const float(&lo)[8] = *reinterpret_cast<const float(*)[8]>(&x[0]);
-            const float(&hi)[8] = *reinterpret_cast<const float(*)[8]>(&x[8]);
-            reinterpret_cast<uint4*>(dst)[sub] = pack8<T>(lo);
-            reinterpret_cast<uint4*>(dst)[LPR + sub] = pack8<T>(hi);
-        }
-    };
     for (int h = h0; h < h1; ++h) {
-        uint4 klo = make_uint4(0, 0, 0, 0), khi = klo, vlo = klo, vhi = klo;
+        typename R::Words kw = {}, vw = {};
         if (valid) {
-            const uint4* k4 = reinterpret_cast<const uint4*>(kb + h * a.k_sh);
-            const uint4* v4 = reinterpret_cast<const uint4*>(vb + h * a.v_sh);
-            klo = __ldcs(k4 + sub);
-            khi = __ldcs(k4 + LPR + sub);
-            vlo = __ldcs(v4 + sub);
-            vhi = __ldcs(v4 + LPR + sub);
+            R::template load<true>(kw, kb + h * a.k_sh, sub);
+            R::template load<true>(vw, vb + h * a.v_sh, sub);
         }
-        float x[16];
-        unpack8<T>(klo, *reinterpret_cast<float(*)[8]>(&x[0]));
-        unpack8<T>(khi, *reinterpret_cast<float(*)[8]>(&x[8]));
-        if (a.gamma != nullptr) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-            for (int m = LPR / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            const float inv = rsqrtf(ss * (1.0f / static_cast<float>(D)) + a.eps);
-            float g[16];
-            unpack8<T>(glo, *reinterpret_cast<float(*)[8]>(&g[0]));
-            unpack8<T>(ghi, *reinterpret_cast<float(*)[8]>(&g[8]));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * g[i];
-        }
-        if (rope) {
-            float cl[8], ch[8], sl[8], sh[8];
-            unpack8<T>(clo, cl);
-            unpack8<T>(chi, ch);
-            unpack8<T>(slo, sl);
-            unpack8<T>(shi, sh);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float lo = x[i], hi = x[8 + i];
-                x[i] = lo * cl[i] - hi * sl[i];
-                x[8 + i] = hi * ch[i] + lo * sh[i];
-            }
-        }
-        const long long ks = E8 ? page * a.c.ks_sp + h * a.c.ks_sh + row : 0;
-        const long long vs = E8 ? page * a.c.vs_sp + h * a.c.vs_sh + row : 0;
-        if constexpr (!E8) {
-            put(x, kd + h * a.c.k_sh, nullptr);
-            if (valid) {
-                reinterpret_cast<uint4*>(vd + h * a.c.v_sh)[sub] = vlo;
-                reinterpret_cast<uint4*>(vd + h * a.c.v_sh)[LPR + sub] = vhi;
-            }
-        } else {
-            put(x, kd + h * a.c.k_sh, a.c.k_scale + ks);
-            unpack8<T>(vlo, *reinterpret_cast<float(*)[8]>(&x[0]));
-            unpack8<T>(vhi, *reinterpret_cast<float(*)[8]>(&x[8]));
-            put(x, vd + h * a.c.v_sh, a.c.v_scale + vs);
+        R k, v;
+        k.template unpack<T>(kw);
+        v.template unpack<T>(vw);
+        if (a.gamma != nullptr) k.template norm<T>(gamma, a.eps);
+        if (a.cos != nullptr) k.template rotate<T>(cos, sin);
+        auto to = [&](unsigned char* dst) {
+            return [=](int at, auto value) {
+                if (valid) *reinterpret_cast<decltype(value)*>(dst + at) = value;
+            };
+        };
+        const uint32_t ke = k.template store<T, E8>(sub, to(kd + h * a.c.k_sh));
+        const uint32_t ve = v.template store<T, E8>(sub, to(vd + h * a.c.v_sh));
+        if (E8 && valid && sub == 0) {
+            a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + row] = static_cast<unsigned char>(ke);
+            a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + row] = static_cast<unsigned char>(ve);
         }
     }
 }

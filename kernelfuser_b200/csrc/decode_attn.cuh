@@ -21,6 +21,8 @@
 // that are loaded while the item before is computed.
 // The exponentials are taken against a base that is only moved when a score exceeds it by more than 2^8 (exact after the
 // division by the sum): as a rule no lane waits for a maximum over lanes.
+// A new token's K and V rows are prepared by the warp that has their step, which puts them into the cache and, for itself,
+// behind the step's cached rows in shared memory: nobody else reads them, so nobody has to wait.
 // Rounding: q' and the probabilities enter the products as the sum of two 16-bit numbers, so that what is left of them is
 // 2^-16 (bf16) or 2^-22 (fp16) of each: a single rounding there doubled the error of a bf16 result (1.6e-3 -> 3.1e-3
 // relative), and the products wait for HBM anyway.  Scores, sums and outputs are 32 bits.  An e4m3 cache is widened to f16
@@ -40,6 +42,8 @@ struct DecodeArgs {
     void* out;
     long long q_sb, q_sh, o_sb, o_sh;   // element strides
     const int* lengths;
+    const void *new_k, *new_v, *gamma_k;  // the newest token's rows, not in the cache yet; null: they are
+    long long nk_sb, nk_sh, nv_sb, nv_sh;
     float* ws;                          // decode_workspace_floats() floats
     unsigned int* arrived;              // a word per CTA, zero before and after the launch (see join_words)
     int B, Hkv, G, row_blocks;          // G query heads per KV head in row_blocks blocks
@@ -51,7 +55,8 @@ struct DecodeArgs {
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;                    // keys of a warp's step
 constexpr int kDecUnit = kDecKeys * kDecWarps;  // keys of a unit
-constexpr int kDecMinUnits = 4;                 // a CTA's piece is at least this long
+// A CTA's piece is at least this many units, or the average item: a join costs about as much as four units of one warp each.
+constexpr int kDecMinUnits = 4;
 
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
@@ -62,12 +67,13 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kCtasPerSm = kQueryInRegs ? 2 : 1;
     // slots of a warp's ring: 100 KB per CTA, as far as two of them fit an SM
     static constexpr int kSlots = E8 ? (D == 128 ? 10 : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
-    static constexpr int kMergeCols = 128, kPad = kMergeCols + 4;     // columns that meet at a time; a row in shared memory
+    static constexpr int kMergeCols = D == 256 && !E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
     static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
     static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kDecWarps + 1) * kRows * 4;
-    static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes;
+    static constexpr int kNewBytes = 2 * kRowBytes;                   // a new token's K and V row
+    static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes + kNewBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
 };
 
@@ -175,97 +181,57 @@ template <typename M, bool FLOOR> __device__ __forceinline__ void split2_probabi
     low = FLOOR ? Num<M>::pack(fmaxf(x, Split<M>::kMin), fmaxf(y, Split<M>::kMin)) : Num<M>::pack(x, y);
 }
 
-// The query rows that a warp prepares for an item (row, row + 4, ...: every lane holds the pairs of columns 2 lane + 64 p
-// and their rotation partners), loaded ahead of time.
+// The query rows that a warp prepares for an item (row, row + 4, ...), loaded ahead of time.
 template <int D, typename T, int NT> struct QueryRows {
-    static constexpr int kPairs = D / 64, kN = 2 * NT;  // pairs of a lane and row; rows of a warp
-    uint32_t q[kN][kPairs], c[kPairs], s[kPairs];
-    __device__ __forceinline__ void load(const DecodeArgs& a, int b, int hk, int len) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = hk / a.row_blocks;
-        const int row0 = (hk - h * a.row_blocks) * 8 * NT;
+    using R = Row<D, 32>;
+    static constexpr int kN = 2 * NT;  // rows of a warp
+    typename R::Words q[kN], cos, sin;
+    __device__ __forceinline__ void load(const DecodeArgs& a, const DecodeCursor& at) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = (at.hk - at.h * a.row_blocks) * 8 * NT;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const int r = row0 + warp + 4 * i;
-            const uint32_t* const src = reinterpret_cast<const uint32_t*>(
-                reinterpret_cast<const T*>(a.q) + b * a.q_sb + (h * a.G + r) * a.q_sh) + lane;
+            if (r < a.G) {
+                R::template load<false>(q[i], reinterpret_cast<const T*>(a.q) + at.b * a.q_sb + (at.h * a.G + r) * a.q_sh, lane);
+            } else {
 #pragma unroll
-            for (int p = 0; p < kPairs; ++p) q[i][p] = r < a.G ? __ldg(src + 32 * p) : 0u;
+                for (int p = 0; p < R::kWords; ++p) q[i][0][p] = q[i][1][p] = 0u;
+            }
         }
         if (a.cos != nullptr) {
-            const long long at = static_cast<long long>(min(len, a.n_pos) - 1) * (D / 2) + lane;
-#pragma unroll
-            for (int p = 0; p < kPairs; ++p) {
-                c[p] = __ldg(reinterpret_cast<const uint32_t*>(a.cos) + at + 32 * p);
-                s[p] = __ldg(reinterpret_cast<const uint32_t*>(a.sin) + at + 32 * p);
-            }
+            const long long row = static_cast<long long>(min(at.len, a.n_pos) - 1) * D;
+            R::template load<false>(cos, reinterpret_cast<const T*>(a.cos) + row, lane);
+            R::template load<false>(sin, reinterpret_cast<const T*>(a.sin) + row, lane);
         }
     }
     // Norm, rotation, and the fragments of the products into shared memory: lane l of a fragment holds row l/4, and of 16
     // columns 2t, 2t+1, 2t+8, 2t+9 (16-bit cache) or 4t .. 4t+3 (8-bit), t = l%4, as a K fragment of that step does.
     // back[row]: what the row's scores are to be multiplied with to undo the scaling of its values (8-bit cache).
-    template <bool E8> __device__ __forceinline__ void prepare(const DecodeArgs& a, const uint32_t (&gamma)[kPairs], uint4* frag, float* back) const {
+    template <bool E8> __device__ __forceinline__ void prepare(const DecodeArgs& a, const typename R::Words& gamma, uint4* frag, float* back) const {
         using M = typename std::conditional<E8, __half, T>::type;
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            float x[kPairs][2];
-#pragma unroll
-            for (int p = 0; p < kPairs; ++p) {
-                const float2 v = Num<T>::unpack(q[i][p]);
-                x[p][0] = v.x;
-                x[p][1] = v.y;
-            }
-            if (a.gamma != nullptr) {
-                float ss = 0.f;
-#pragma unroll
-                for (int p = 0; p < kPairs; ++p) ss = fmaf(x[p][0], x[p][0], fmaf(x[p][1], x[p][1], ss));
-#pragma unroll
-                for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-                const float inv = rsqrtf(ss * (1.0f / static_cast<float>(D)) + a.eps);
-#pragma unroll
-                for (int p = 0; p < kPairs; ++p) {
-                    const float2 v = Num<T>::unpack(gamma[p]);
-                    x[p][0] = x[p][0] * inv * v.x;
-                    x[p][1] = x[p][1] * inv * v.y;
-                }
-            }
-            if (a.cos != nullptr) {
-#pragma unroll
-                for (int p = 0; p < kPairs / 2; ++p) {
-                    constexpr int kP = kPairs / 2;
-                    const float2 cl = Num<T>::unpack(c[p]), ch = Num<T>::unpack(c[p + kP]);
-                    const float2 sl = Num<T>::unpack(s[p]), sh = Num<T>::unpack(s[p + kP]);
-                    const float lo0 = x[p][0], lo1 = x[p][1], hi0 = x[p + kP][0], hi1 = x[p + kP][1];
-                    x[p][0] = lo0 * cl.x - hi0 * sl.x;
-                    x[p][1] = lo1 * cl.y - hi1 * sl.y;
-                    x[p + kP][0] = hi0 * ch.x + lo0 * sh.x;
-                    x[p + kP][1] = hi1 * ch.y + lo1 * sh.y;
-                }
-            }
             const int r = warp + 4 * i;
-            if constexpr (E8) {
-                uint32_t amax = 0;
-#pragma unroll
-                for (int p = 0; p < kPairs; ++p)
-                    amax = max(amax, max(__float_as_uint(x[p][0]) & 0x7fffffffu, __float_as_uint(x[p][1]) & 0x7fffffffu));
-                amax = __reduce_max_sync(0xffffffffu, amax);
-                // largest value to [2^14, 2^15) (an infinity or a NaN stays what it is)
-                const uint32_t e = min(max(amax >> 23, 15u), 254u);
-                const float up = __uint_as_float((268u - e) << 23);                    // 2^(141 - e)
+            R row;
+            row.template unpack<T>(q[i]);
+            if (a.gamma != nullptr) row.template norm<T>(gamma, a.eps);
+            if (a.cos != nullptr) row.template rotate<T>(cos, sin);
+            float up = 1.f;
+            if constexpr (E8) {  // largest value to [2^14, 2^15) (an infinity or a NaN stays what it is)
+                const uint32_t e = min(max(row.largest() >> 23, 15u), 254u);
+                up = __uint_as_float((268u - e) << 23);                                     // 2^(141 - e)
                 if (lane == 0) back[r] = a.scale_log2e * __uint_as_float((e - 14u) << 23);  // 2^(e - 141)
+            }
 #pragma unroll
-                for (int p = 0; p < kPairs; ++p) {
-                    x[p][0] *= up;
-                    x[p][1] *= up;
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int p = 0; p < R::kWords; ++p) {
+                    const int col = half * (D / 2) + lane * R::W + 2 * p, in = col % 16;
+                    const int t = E8 ? in / 4 : in % 8 / 2, reg = E8 ? in % 4 / 2 : in / 8;
+                    uint32_t* const dst = reinterpret_cast<uint32_t*>(frag + (r / 8 * (D / 16) + col / 16) * 32 + r % 8 * 4 + t);
+                    split2<M>(row.x[half][2 * p] * up, row.x[half][2 * p + 1] * up, dst[reg], dst[reg + 2]);
                 }
-            }
-#pragma unroll
-            for (int p = 0; p < kPairs; ++p) {
-                const int col = 2 * lane + 64 * p, in = col % 16;
-                const int t = E8 ? in / 4 : in % 8 / 2, reg = E8 ? in % 4 / 2 : in / 8;
-                uint32_t* const dst = reinterpret_cast<uint32_t*>(frag + (r / 8 * (D / 16) + col / 16) * 32 + r % 8 * 4 + t);
-                split2<M>(x[p][0], x[p][1], dst[reg], dst[reg + 2]);
-            }
         }
     }
 };
@@ -284,89 +250,113 @@ template <int D, bool E8, int NT> __host__ __device__ constexpr long long decode
 // (8-15), and joined groups of the item that begins in it (16-31).  Who completes a field takes it back to zero.
 constexpr int kJoin = 16;
 
+struct DecodeBroken {
+    int first, last;  // its CTAs; first < 0: there is none
+    int b, hk, h;
+};
+
 template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     using C = DecodeCfg<D, E8, NT>;
     static constexpr int kRows = C::kRows;
     const DecodeArgs& a;
-    float* scratch;  // shared memory: maxima and sums of the parts, and of the result
-    int* s_flag;
+    float* scratch;  // shared memory: 2 * kRows
+    int* s_flag;     // shared memory: 2
 
-    // All threads: count one more in the field; true for the CTA that completes `count`.
-    __device__ __forceinline__ bool arrive(int cta, int shift, int count) const {
-        __threadfence();  // the part is visible before it counts
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const unsigned int before = atomicAdd(a.arrived + cta, 1u << shift);
-            const bool all = static_cast<int>(before >> shift & (shift == 16 ? 0xffffu : 0xffu)) == count - 1;
-            if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
-            __threadfence();
-            *s_flag = all;
-        }
-        __syncthreads();
-        return *s_flag != 0;
+    // One thread: count one more in the field; true for the CTA that completes `count`.
+    __device__ __forceinline__ bool count_up(int cta, int shift, int count) const {
+        const unsigned int before = atomicAdd(a.arrived + cta, 1u << shift);
+        const bool all = static_cast<int>(before >> shift & (shift == 16 ? 0xffffu : 0xffu)) == count - 1;
+        if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
+        return all;
     }
-    // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.
+    // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.  A
+    // thread takes four columns of a row; it loads eight parts at a time and keeps their maximum and sum itself.
     __device__ __forceinline__ void sum(int first, int from, int stride, int n, float* out, int b, int h, int row0) const {
-        float* const top = scratch;
-        float* const total = top + kRows;
-        float* const m = total + kRows;  // [n][kRows]
-        float* const l = m + n * kRows;
-        auto part = [&](int i) { return a.ws + decode_part_at<D, E8, NT>(from + i * stride, from + i * stride == first); };
-        for (int i = threadIdx.x; i < n * kRows; i += kDecThreads) {
-            m[i] = __ldcg(part(i / kRows) + kRows * D + i % kRows);
-            l[i] = __ldcg(part(i / kRows) + kRows * D + kRows + i % kRows);
-        }
-        __syncthreads();
-        if (threadIdx.x < kRows) {
-            const int r = threadIdx.x;
-            float t = -INFINITY, s = 0.f;
-            for (int i = 0; i < n; ++i) t = fmaxf(t, m[i * kRows + r]);
-            for (int i = 0; i < n; ++i) {
-                const float f = m[i * kRows + r] == -INFINITY ? 0.f : exp2f(m[i * kRows + r] - t);
-                s += l[i * kRows + r] * f;
-                m[i * kRows + r] = f;
-            }
-            top[r] = t;
-            total[r] = s;
-        }
-        __syncthreads();
+        constexpr int kAtOnce = 8;
         for (int e = threadIdx.x; e < kRows * (D / 4); e += kDecThreads) {
             const int r = e / (D / 4), d = (e % (D / 4)) * 4;
             if (row0 + r >= a.G) break;  // (rows go up with e)
             float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(part(i) + r * D + d));
-                const float f = m[i * kRows + r];
-                z.x += x.x * f;
-                z.y += x.y * f;
-                z.z += x.z * f;
-                z.w += x.w * f;
+            float top = -INFINITY, total = 0.f;
+            for (int i0 = 0; i0 < n; i0 += kAtOnce) {
+                float4 x[kAtOnce];
+                float m[kAtOnce], l[kAtOnce], to = top;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int cta = from + min(i0 + i, n - 1) * stride;
+                    const float* const part = a.ws + decode_part_at<D, E8, NT>(cta, cta == first);
+                    x[i] = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
+                    m[i] = __ldcg(part + kRows * D + r);
+                    l[i] = __ldcg(part + kRows * D + kRows + r);
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, m[i]);
+                const float f = top == -INFINITY ? 0.f : exp2f(top - to);
+                z = make_float4(z.x * f, z.y * f, z.z * f, z.w * f);
+                total *= f;
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+                    if (i0 + i < n) {
+                        const float w = m[i] == -INFINITY ? 0.f : exp2f(m[i] - to);
+                        z = make_float4(z.x + x[i].x * w, z.y + x[i].y * w, z.z + x[i].z * w, z.w + x[i].w * w);
+                        total += l[i] * w;
+                    }
+                top = to;
             }
             if (out != nullptr) {
+                // (in place of the part that this very thread has read; its maximum and sum are still read by others)
                 *reinterpret_cast<float4*>(out + r * D + d) = z;
-                if (d == 0) {
-                    out[kRows * D + r] = top[r];
-                    out[kRows * D + kRows + r] = total[r];
-                }
             } else {
                 T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
-                const float inv = 1.f / total[r];
+                const float inv = 1.f / total;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
             }
+            if (d == 0) {
+                scratch[r] = top;
+                scratch[kRows + r] = total;
+            }
+        }
+        if (out == nullptr) return;
+        __syncthreads();
+        if (threadIdx.x < kRows && row0 + threadIdx.x < a.G) {
+            out[kRows * D + threadIdx.x] = scratch[threadIdx.x];
+            out[kRows * D + kRows + threadIdx.x] = scratch[kRows + threadIdx.x];
+        }
+    }
+    // All threads, once: this CTA's parts are in their places (`dead`: they never will be; only the counts have to go on).
+    __device__ __forceinline__ void parts_done(const DecodeBroken (&item)[2], bool dead) const {
+        const int cta = blockIdx.x;
+        __threadfence();  // the parts are visible before they count
+        __syncthreads();
+        if (threadIdx.x == 0 || threadIdx.x == 32) {  // (a lane of its own for each: the two round trips overlap)
+            const DecodeBroken& it = item[threadIdx.x / 32];
+            bool all = false;
+            if (it.first >= 0) {
+                const int from = it.first + (cta - it.first) / kJoin * kJoin, n = min(kJoin, it.last - from + 1);
+                all = n == 1 || count_up(from, from == it.first ? 8 : 0, n);
+            }
+            __threadfence();
+            s_flag[threadIdx.x / 32] = all;
         }
         __syncthreads();
-    }
-    // This CTA's part of the item is in its place (`dead`: it never will be; only the counts have to go on).
-    __device__ __forceinline__ void part_done(int first, int last, int b, int hk, int h, bool dead) const {
-        const int cta = blockIdx.x, row0 = (hk - h * a.row_blocks) * kRows;
-        const int groups = (last - first) / kJoin + 1, from = first + (cta - first) / kJoin * kJoin;
-        const int n = min(kJoin, last - from + 1);
-        if (n > 1 && !arrive(from, from == first ? 8 : 0, n)) return;
-        float* const place = groups == 1 ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == first);
-        if (n > 1 && !dead) sum(first, from, 1, n, place, b, h, row0);
-        if (groups == 1 || !arrive(first, 16, groups) || dead) return;
-        sum(first, first, kJoin, groups, nullptr, b, h, row0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const DecodeBroken& it = item[k];
+            if (s_flag[k] == 0) continue;
+            const int groups = (it.last - it.first) / kJoin + 1, from = it.first + (cta - it.first) / kJoin * kJoin;
+            const int n = min(kJoin, it.last - from + 1), row0 = (it.hk - it.h * a.row_blocks) * kRows;
+            float* const place = groups == 1 ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == it.first);
+            if (n > 1 && !dead) sum(it.first, from, 1, n, place, it.b, it.h, row0);
+            if (groups == 1) continue;
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                s_flag[k] = count_up(it.first, 16, groups);
+                __threadfence();
+            }
+            __syncthreads();
+            if (s_flag[k] != 0 && !dead) sum(it.first, it.first, kJoin, groups, nullptr, it.b, it.h, row0);
+        }
     }
 };
 
@@ -375,104 +365,77 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     using C = DecodeCfg<D, E8, NT>;
     using M = typename std::conditional<E8, __half, T>::type;  // type of the products' operands
     constexpr int kDT = D / 16, kRows = C::kRows;
-    __shared__ long long s_sum[kDecWarps], s_first;
-    __shared__ int s_b, s_dead, s_flag;
+    __shared__ int s_dead, s_flag[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int HK = a.Hkv * a.row_blocks, n_ctas = gridDim.x;
     if (tid == 0) s_dead = *reinterpret_cast<volatile int*>(a.status);  // (one reading for the whole CTA)
 
-    // ---- this CTA's piece of the line of units
-    const int per_thread = (a.B + kDecThreads - 1) / kDecThreads, b_lo = tid * per_thread;
-    long long mine = 0;
-    for (int b = b_lo; b < min(b_lo + per_thread, a.B); ++b) {
-        const int n = __ldg(a.lengths + b);
-        if (n > a.c.capacity) report(a.status, kStatusBadLength);
-        if (a.cos != nullptr && n > a.n_pos) report(a.status, kStatusBadPosition);
-        mine += units_of(cached_rows(a, b));
-    }
-    long long before = mine;  // inclusive sums within the warp
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += x;
-    }
-    if (lane == 31) s_sum[warp] = before;
-    __syncthreads();
-    const bool dead = s_dead != 0;  // then nothing is read or written but the counts of the joins, which other CTAs may wait for
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-        if (w < warp) before += s_sum[w];
-        total += s_sum[w];
-    }
-    before -= mine;
-    total *= HK;
-    long long piece = (total + n_ctas - 1) / n_ctas;
-    if (piece < kDecMinUnits) piece = kDecMinUnits;
-    const long long u0 = piece * blockIdx.x, u1 = min(u0 + piece, total);
-    if (u0 < total && before * HK <= u0 && u0 < (before + mine) * HK) {  // (one thread of the CTA)
-        int b = b_lo;
-        long long at = before;
-        for (;;) {
-            const int n = units_of(cached_rows(a, b));
-            if (u0 < (at + n) * HK) break;
-            at += n;
-            ++b;
-        }
-        s_b = b;
-        s_first = at;
-    }
-    // sequences without rows have no units: their output is zero
-    for (int b = blockIdx.x; b < a.B && !dead; b += n_ctas)
-        if (cached_rows(a, b) == 0) {
-            const int Hq = a.Hkv * a.G;
-            for (int i = tid; i < Hq * (D / 8); i += kDecThreads)
-                reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
-                    make_uint4(0, 0, 0, 0);
-        }
-    if (u0 >= total) return;
-    __syncthreads();
+    // ---- this CTA's piece of the line of units; each warp finds it for itself
+    unsigned int u0, u1, piece;
     DecodeCursor cc;
-    cc.b = s_b;
-    cc.len = cached_rows(a, cc.b);
-    cc.nt = units_of(cc.len);
     {
-        const long long in_b = u0 - s_first * HK;
-        cc.hk = static_cast<int>(in_b / cc.nt);
-        cc.t = static_cast<int>(in_b - static_cast<long long>(cc.hk) * cc.nt);
-        cc.h = cc.hk / a.row_blocks;
-    }
-    cc.left = static_cast<int>(u1 - u0);
-    // the broken items: the one that began before this piece or fills it, and the one that begins in it and goes on
-    int first0 = -1, last0 = 0, b0 = 0, hk0 = 0, h0 = 0, last1 = -1, b1 = 0, hk1 = 0, h1 = 0;
-    if (cc.t > 0) {
-        first0 = static_cast<int>((u0 - cc.t) / piece);
-        last0 = static_cast<int>((u0 - cc.t + cc.nt - 1) / piece);
-        b0 = cc.b;
-        hk0 = cc.hk;
-        h0 = cc.h;
-    }
-    auto begins_and_goes_on = [&](int n) {  // n units of item cc here
-        if (cc.t > 0 || n == cc.nt) return;
-        last1 = static_cast<int>((u1 - 1 + (cc.nt - n)) / piece);
-        b1 = cc.b;
-        hk1 = cc.hk;
-        h1 = cc.h;
-    };
-    if (dead) {
-        while (cc.left > 0) {
-            const int n = min(cc.nt - cc.t, cc.left);
-            if (n <= 0) break;
-            begins_and_goes_on(n);
-            cc.t += n;
-            cc.left -= n;
-            if (cc.left > 0) cc.next_item(a, HK);
+        const int per_lane = (a.B + 31) / 32, b_lo = lane * per_lane;
+        unsigned int mine = 0, rows_at_all = 0;
+        for (int b = b_lo; b < min(b_lo + per_lane, a.B); ++b) {
+            const int n = __ldg(a.lengths + b);
+            if (n > a.c.capacity) report(a.status, kStatusBadLength);
+            if (a.cos != nullptr && n > a.n_pos) report(a.status, kStatusBadPosition);
+            mine += units_of(min(max(n, 0), a.c.capacity));
+            rows_at_all += n > 0;
         }
-        const DecodeJoin<D, T, E8, NT> join{a, nullptr, &s_flag};
-        if (first0 >= 0) join.part_done(first0, last0, b0, hk0, h0, true);
-        if (last1 >= 0) join.part_done(blockIdx.x, last1, b1, hk1, h1, true);
+        unsigned int before = mine;  // inclusive sums
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const unsigned int x = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += x;
+        }
+        const unsigned int sum = __shfl_sync(0xffffffffu, before, 31), total = sum * HK;  // (the host has seen to it that this fits)
+        const unsigned int average = sum / max(__reduce_add_sync(0xffffffffu, rows_at_all), 1u);
+        piece = max((total + n_ctas - 1) / n_ctas, min(static_cast<unsigned int>(kDecMinUnits), max(average, 1u)));
+        u0 = piece * blockIdx.x;
+        u1 = min(u0 + piece, total);
+        before -= mine;
+        const unsigned int here = __ballot_sync(0xffffffffu, u0 < total && before * HK <= u0 && u0 < (before + mine) * HK);
+        int b = b_lo;
+        if (here >> lane & 1) {
+            for (;;) {
+                const unsigned int n = units_of(cached_rows(a, b));
+                if (u0 < (before + n) * HK) break;
+                before += n;
+                ++b;
+            }
+        }
+        const int src = here == 0 ? 0 : __ffs(here) - 1;
+        cc.b = __shfl_sync(0xffffffffu, b, src);
+        const unsigned int in_b = u0 - __shfl_sync(0xffffffffu, before, src) * HK;
+        cc.left = 0;
+        if (here != 0) {
+            cc.len = cached_rows(a, cc.b);
+            cc.nt = units_of(cc.len);
+            cc.hk = in_b / cc.nt;
+            cc.t = in_b - cc.hk * cc.nt;
+            cc.h = cc.hk / a.row_blocks;
+            cc.left = u1 - u0;
+        }
+    }
+    auto empty_rows = [&] {  // sequences without rows have no units: their output is zero
+        for (int b = blockIdx.x; b < a.B; b += n_ctas)
+            if (cached_rows(a, b) == 0)
+                for (int i = tid; i < a.Hkv * a.G * (D / 8); i += kDecThreads)
+                    reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
+                        make_uint4(0, 0, 0, 0);
+    };
+    if (cc.left == 0) {  // (all warps of the CTA alike)
+        __syncthreads();
+        if (s_dead == 0) empty_rows();
         return;
     }
+    // the broken items: the one that began before this piece (or fills it), and the one that begins in it and goes on
+    DecodeBroken broken[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};
+    if (cc.t > 0) broken[0] = {static_cast<int>((u0 - cc.t) / piece), static_cast<int>((u0 - cc.t + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
+    auto begins_and_goes_on = [&](int n) {  // n units of item cc are here
+        if (cc.t == 0 && n < cc.nt) broken[1] = {static_cast<int>(blockIdx.x), static_cast<int>((u1 - 1 + (cc.nt - n)) / piece), cc.b, cc.hk, cc.h};
+    };
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
     // eight rows of a column block lie in different banks)
@@ -484,14 +447,13 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     float* const merge_m = merge_o + 2 * 8 * C::kPad;                                        // [warps][rows]
     float* const merge_l = merge_m + kDecWarps * kRows;
     float* const back = merge_l + kDecWarps * kRows;                                         // [rows]
+    unsigned char* const new_rows = smem + C::kSmemBytes - C::kScaleRingBytes - C::kNewBytes;  // K and V row of a new token
 
     QueryRows<D, T, NT> rows;
-    rows.load(a, cc.b, cc.hk, cc.len);
-    uint32_t gamma[D / 64];
-    if (a.gamma != nullptr) {
-#pragma unroll
-        for (int p = 0; p < D / 64; ++p) gamma[p] = __ldg(reinterpret_cast<const uint32_t*>(a.gamma) + lane + 32 * p);
-    }
+    using R = Row<D, 32>;
+    rows.load(a, cc);
+    typename R::Words gamma;
+    if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, lane);
 
     DecodeCursor pc = cc;
     int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
@@ -503,8 +465,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     // 16 rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
     auto copy_rows = [&](int slot, const unsigned char* pool, long long sp, long long sh, long long ss, const unsigned char* scale,
                          long long scale_sp, long long scale_sh) {
-        const int n = pc.len - (pc.t * kDecUnit + warp * kDecKeys);
+        int n = pc.len - (pc.t * kDecUnit + warp * kDecKeys);
         if (n <= 0 || page < 0) return;
+        n -= a.new_k != nullptr;  // (the last row is not in the cache yet)
         const unsigned char* const src = pool + page * sp + pc.h * sh + (row0_in_page + r_lane) * ss + piece16 * 16;
         const uint32_t base = dst_lane + slot * C::kSlotBytes;
         auto dst = [&](int i) {  // row r_lane + i * kRowsAtOnce (r_lane is below kRowsAtOnce, a power of two)
@@ -559,10 +522,10 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         }
         cp_async_commit();
     };
-#pragma unroll
-    for (int s = 0; s < C::kSlots - 1; ++s) {
-        if (s % 2 == 0) issue_k(s);
-        else issue_v(s);
+#pragma unroll 1
+    for (int s = 0; s < C::kSlots - 1; s += 2) {
+        issue_k(s);
+        if (s + 1 < C::kSlots - 1) issue_v(s + 1);
     }
     // A step's two halves: wait for the slot, refill the one before it, which all lanes are done with.
     int slot = 0;
@@ -578,6 +541,67 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
 
     rows.template prepare<E8>(a, gamma, frag, back);
     __syncthreads();
+    if (s_dead != 0) {  // nothing is written; only the joins are counted on, other CTAs may complete them
+        cp_async_wait<0>();
+        while (cc.left > 0) {
+            const int n = min(cc.nt - cc.t, cc.left);
+            if (n <= 0) break;
+            begins_and_goes_on(n);
+            cc.t += n;
+            cc.left -= n;
+            if (cc.left > 0) cc.next_item(a, HK);
+        }
+        DecodeJoin<D, T, E8, NT>{a, nullptr, s_flag}.parts_done(broken, true);
+        return;
+    }
+    empty_rows();
+
+    // The new token's rows of an item, by the warp that has their step: into the cache and into new_rows.
+    uint32_t new_ke = 0, new_ve = 0;  // scales' bytes
+    auto prepare_new = [&] {
+        const int pos = cc.len - 1, i = pos / a.c.page_size, row = pos - i * a.c.page_size;
+        typename R::Words kw, vw, gk, c, s;
+        const int pg = __ldg(a.c.pages + cc.b * a.c.pages_sb + i);
+        R::template load<false>(kw, reinterpret_cast<const T*>(a.new_k) + cc.b * a.nk_sb + cc.h * a.nk_sh, lane);
+        R::template load<false>(vw, reinterpret_cast<const T*>(a.new_v) + cc.b * a.nv_sb + cc.h * a.nv_sh, lane);
+        if (a.gamma_k != nullptr) R::template load<false>(gk, a.gamma_k, lane);
+        bool write = cc.hk == cc.h * a.row_blocks && __ldg(a.lengths + cc.b) <= a.c.capacity;
+        if (a.cos != nullptr) {
+            write = write && pos < a.n_pos;
+            const long long at = static_cast<long long>(min(pos, a.n_pos - 1)) * D;
+            R::template load<false>(c, reinterpret_cast<const T*>(a.cos) + at, lane);
+            R::template load<false>(s, reinterpret_cast<const T*>(a.sin) + at, lane);
+        }
+        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) write = false;  // (reported by the copies of the step)
+        R k, v;
+        k.template unpack<T>(kw);
+        v.template unpack<T>(vw);
+        if (a.gamma_k != nullptr) k.template norm<T>(gk, a.eps);
+        if (a.cos != nullptr) k.template rotate<T>(c, s);
+        auto to = [&](unsigned char* dst, unsigned char* pool) {
+            return [=](int at, auto value) {
+                *reinterpret_cast<decltype(value)*>(dst + at) = value;
+                if (write) *reinterpret_cast<decltype(value)*>(pool + at) = value;
+            };
+        };
+        const long long p = write ? pg : 0;
+        new_ke = k.template store<T, E8>(lane, to(new_rows, a.c.k + p * a.c.k_sp + cc.h * a.c.k_sh + row * a.c.k_ss));
+        new_ve = v.template store<T, E8>(lane, to(new_rows + C::kRowBytes, a.c.v + p * a.c.v_sp + cc.h * a.c.v_sh + row * a.c.v_ss));
+        if (E8 && write && lane == 0) {
+            a.c.k_scale[p * a.c.ks_sp + cc.h * a.c.ks_sh + row] = static_cast<unsigned char>(new_ke);
+            a.c.v_scale[p * a.c.vs_sp + cc.h * a.c.vs_sh + row] = static_cast<unsigned char>(new_ve);
+        }
+        __syncwarp();
+    };
+    // and from there behind the cached rows of the step in `slot`
+    auto place_new = [&](int slot, int v) {
+        const int r = (cc.len - 1) % kDecKeys;
+        if (lane < kPieces)
+            *reinterpret_cast<uint4*>(smem + (warp * C::kSlots + slot) * C::kSlotBytes + r * C::kRowBytes + ((lane ^ (r & 7)) << 4)) =
+                *reinterpret_cast<const uint4*>(new_rows + v * C::kRowBytes + lane * 16);
+        if (E8 && lane == 0) scales[slot * kDecKeys + r] = static_cast<unsigned char>(v ? new_ve : new_ke);
+        __syncwarp();
+    };
 
     // ldmatrix: the row (key) of the slot and the 16-byte piece that this lane names; piece + 2 j lies 32 j bytes further,
     // xor-ed below 128 bytes
@@ -604,7 +628,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         nc.left -= n;
         if (nc.left > 0) {
             nc.next_item(a, HK);
-            rows.load(a, nc.b, nc.hk, nc.len);
+            rows.load(a, nc);
         }
         uint4 qf[C::kQueryInRegs ? NT : 1][C::kQueryInRegs ? kDT : 1];
         if constexpr (C::kQueryInRegs) {
@@ -630,10 +654,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             off[u][0] = off[u][1] = off_v[u][0] = off_v[u][1] = 0.f;
             l[u][0] = l[u][1] = 0.f;
         }
+        // the new token's step is the last one with keys, in the item's last unit
+        const bool has_new = a.new_k != nullptr && cc.t + n == cc.nt && warp == (cc.len - 1) % kDecUnit / kDecKeys;
+        if (has_new) prepare_new();
         for (int i_unit = 0; i_unit < n; ++i_unit) {
             const int keys = cc.len - ((cc.t + i_unit) * kDecUnit + warp * kDecKeys);  // of the sequence, from this step's first on
             arrive(std::false_type{});
             float x[NT][4], w[NT][4];  // scores of keys g (0, 1), g + 8 (2, 3) and heads 2 t4, 2 t4 + 1
+            if (has_new && i_unit == n - 1) place_new(slot, 0);
             if (keys > 0) {
                 float s[NT][2][4];  // high and low part of q': two chains of products
 #pragma unroll
@@ -687,6 +715,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             }
             leave();
             arrive(std::true_type{});
+            if (has_new && i_unit == n - 1) place_new(slot, 1);
             if (keys > 0) {
                 bool above = false;
                 if constexpr (E8) {
@@ -822,7 +851,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         begins_and_goes_on(n);
         float* const part = a.ws + decode_part_at<D, E8, NT>(blockIdx.x, cc.t == 0 ? 1 : 0);
         float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
-        // eight rows and 128 columns at a time: warps 2 and 3 leave theirs, 0 and 1 add theirs, all add the two copies
+        // eight rows and kMergeCols columns at a time: warps 2 and 3 leave theirs, 0 and 1 add theirs, all add the two copies
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -869,11 +898,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             }
         cc = nc;
     }
-    cp_async_wait<0>();
-    __syncthreads();  // (the ring serves the joins)
-    const DecodeJoin<D, T, E8, NT> join{a, reinterpret_cast<float*>(smem), &s_flag};
-    if (first0 >= 0) join.part_done(first0, last0, b0, hk0, h0, false);
-    if (last1 >= 0) join.part_done(blockIdx.x, last1, b1, hk1, h1, false);
+    cp_async_wait<0>();  // (the ring's first bytes serve the joins)
+    DecodeJoin<D, T, E8, NT>{a, reinterpret_cast<float*>(smem), s_flag}.parts_done(broken, false);
 }
 
 }  // namespace kf

@@ -141,8 +141,9 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     // no more CTAs than the batch can have pieces of work
     const long long most = static_cast<long long>(a.B) * a.Hkv * args.row_blocks *
                            ((a.c.capacity + kf::kDecUnit - 1) / kf::kDecUnit);
-    const long long want = (most + kf::kDecMinUnits - 1) / kf::kDecMinUnits, fit = decode_ctas<D, E8, NT>();
-    const unsigned grid = (unsigned)(want < fit ? want : fit);
+    if (most > 0x7fffffffLL) return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
+    const long long fit = decode_ctas<D, E8, NT>();
+    const unsigned grid = (unsigned)(most < fit ? most : fit);
     if (grid > 1) {
         if (int r = join_words(st, &args.arrived)) return r;
         if (args.arrived == nullptr) {  // then words in the workspace, cleared by the graph itself
@@ -268,17 +269,8 @@ int kf_decode_attention(const kf_decode_params* p, void* stream) {
         if (!aligned16(p->gamma_k)) return fail(KF_EALIGN, "pointers must be 16-byte aligned");
     }
     if (int r = check_device()) return r;
-    if (p->new_k) {
-        kf::AppendArgs n{};
-        n.c = a.c;
-        n.k = p->new_k; n.v = p->new_v; n.gamma = p->gamma_k; n.cos = p->cos_table; n.sin = p->sin_table;
-        n.k_sb = p->k_stride_b; n.k_sh = p->k_stride_h; n.v_sb = p->v_stride_b; n.v_sh = p->v_stride_h;
-        n.start = p->lengths; n.newest = 1;
-        n.B = (int)p->B; n.H = (int)Hkv; n.S = 1; n.n_pos = (int)p->n_positions;
-        n.eps = (float)p->eps;
-        n.status = p->status;
-        if (int r = by_type(D, p->dtype, p->cache.dtype == KF_E4M3, Append{n, st})) return r;
-    }
+    a.new_k = p->new_k; a.new_v = p->new_v; a.gamma_k = p->gamma_k;
+    a.nk_sb = p->k_stride_b; a.nk_sh = p->k_stride_h; a.nv_sb = p->v_stride_b; a.nv_sh = p->v_stride_h;
     a.q = p->q; a.gamma = p->gamma_q; a.cos = p->cos_table; a.sin = p->sin_table;
     a.out = p->out;
     a.q_sb = p->q_stride_b; a.q_sh = p->q_stride_h; a.o_sb = p->o_stride_b; a.o_sh = p->o_stride_h;
