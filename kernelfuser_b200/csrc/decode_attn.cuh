@@ -10,7 +10,7 @@
 // every CTA takes an equal piece of it, found from the lengths on the device: ragged batches and single long sequences
 // load all SMs alike, and a captured launch follows its lengths.  A CTA's piece covers whole (sequence, head) items and
 // at most two broken ones; a broken item's parts meet in the workspace, where the CTA that comes last joins them, in the
-// order of the line whoever that is: 16 at a time, and if there are more, the joined sixteens once more.  (A second kernel
+// order of the line whoever that is: as many at a time as its ring holds, and if there are more, the joined groups once more.  (A second kernel
 // for it cost 2 us of a call, and its serial pass over 37 parts of a long sequence 12 us.)
 //
 // Inside a CTA each of the four warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
@@ -58,15 +58,23 @@ constexpr int kDecUnit = kDecKeys * kDecWarps;  // keys of a unit
 // A CTA's piece is at least this many units, or the average item: a join costs about as much as four units of one warp each.
 constexpr int kDecMinUnits = 4;
 
+#ifndef KF_E8_CTAS
+#define KF_E8_CTAS 3
+#define KF_E8_SLOTS 7
+#endif
+#ifndef KF_ITEM_COST
+#define KF_ITEM_COST 1
+#endif
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
+    static constexpr int kItemCost = KF_ITEM_COST;
     static constexpr int kRowBytes = D * (E8 ? 1 : 2);
     static constexpr int kSlotBytes = kDecKeys * kRowBytes;           // K or V rows of a step
     static constexpr int kScaleBytes = E8 ? kDecKeys : 0;             // and their scales
     static constexpr bool kQueryInRegs = D * NT <= 256;               // else its fragments are read for every step
-    static constexpr int kCtasPerSm = kQueryInRegs ? 2 : 1;
+    static constexpr int kCtasPerSm = E8 && D == 128 && NT == 1 ? KF_E8_CTAS : kQueryInRegs ? 2 : 1;
     // slots of a warp's ring: 100 KB per CTA, as far as two of them fit an SM
-    static constexpr int kSlots = E8 ? (D == 128 ? 10 : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
+    static constexpr int kSlots = E8 ? (D == 128 ? (NT == 1 ? KF_E8_SLOTS : 10) : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
     static constexpr int kMergeCols = D == 256 && !E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
     static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
@@ -77,12 +85,23 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+// Copies of cache rows into shared memory.  Each row is read once, so it is the first to leave L2 again: what is read over and
+// over (the kernel's own instructions, weights, tables) stays.
+__device__ __forceinline__ uint64_t evict_first_policy() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+// (without a policy: together with a source size it raised an illegal instruction on B200)
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool take) {
     const int n = take ? 16 : 0;  // (0: zeros, nothing is read)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -123,11 +142,13 @@ __device__ __forceinline__ int cached_rows(const DecodeArgs& a, int b) { return 
 __device__ __forceinline__ int units_of(int len) { return (len + kDecUnit - 1) / kDecUnit; }
 
 // A place in the line of units: unit t of nt of item hk of sequence b.
-struct DecodeCursor {
+template <int COST> struct DecodeCursor {
     int b, hk, h, t, nt, len;
-    int left;  // units up to the end of the CTA's piece
-    // to the next item; only called with units left
+    int left;  // of the line up to the end of the CTA's piece
+    // to the next item, if the piece reaches it
     __device__ __forceinline__ void next_item(const DecodeArgs& a, int HK) {
+        left -= COST;
+        if (left <= 0) return;
         t = 0;
         ++hk;
         h = hk / a.row_blocks;
@@ -186,7 +207,7 @@ template <int D, typename T, int NT> struct QueryRows {
     using R = Row<D, 32>;
     static constexpr int kN = 2 * NT;  // rows of a warp
     typename R::Words q[kN], cos, sin;
-    __device__ __forceinline__ void load(const DecodeArgs& a, const DecodeCursor& at) {
+    template <typename Cursor> __device__ __forceinline__ void load(const DecodeArgs& a, const Cursor& at) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = (at.hk - at.h * a.row_blocks) * 8 * NT;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
@@ -245,11 +266,9 @@ template <int D, bool E8, int NT> __host__ __device__ constexpr long long decode
     return decode_part_at<D, E8, NT>(ctas, 0) + ctas;
 }
 
-// Joining.  Item parts of CTAs first .. last (one that begins in `first`); groups of kJoin consecutive ones.  A CTA's word
-// counts in three fields: parts that have arrived of the group whose first part is its part 0 (bits 0-7) or its part 1
+// Joining.  Item parts of CTAs first .. last (one that begins in `first`); groups of join_group() consecutive ones.  A CTA's
+// word counts in three fields: parts that have arrived of the group whose first part is its part 0 (bits 0-7) or its part 1
 // (8-15), and joined groups of the item that begins in it (16-31).  Who completes a field takes it back to zero.
-constexpr int kJoin = 16;
-
 struct DecodeBroken {
     int first, last;  // its CTAs; first < 0: there is none
     int b, hk, h;
@@ -259,8 +278,12 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     using C = DecodeCfg<D, E8, NT>;
     static constexpr int kRows = C::kRows;
     const DecodeArgs& a;
-    float* scratch;  // shared memory: 2 * kRows
+    float* room;     // shared memory: the ring
     int* s_flag;     // shared memory: 2
+
+    // parts that the ring holds side by side, of rows that exist
+    __device__ __forceinline__ int part_floats() const { return min(kRows, a.G) * D + 2 * kRows; }
+    __device__ __forceinline__ int join_group() const { return min(64, C::kRingBytes / 4 / part_floats()); }
 
     // One thread: count one more in the field; true for the CTA that completes `count`.
     __device__ __forceinline__ bool count_up(int cta, int shift, int count) const {
@@ -269,93 +292,116 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
         if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
         return all;
     }
-    // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.  A
-    // thread takes four columns of a row; it loads eight parts at a time and keeps their maximum and sum itself.
+    // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.  The
+    // parts are copied into the ring, then a thread takes four columns of a row.  (Little code: it is run once a launch, and
+    // its own way from memory costs more than what it does: with eight parts at a time in registers 4 us.)
     __device__ __forceinline__ void sum(int first, int from, int stride, int n, float* out, int b, int h, int row0) const {
-        constexpr int kAtOnce = 8;
-        for (int e = threadIdx.x; e < kRows * (D / 4); e += kDecThreads) {
-            const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-            if (row0 + r >= a.G) break;  // (rows go up with e)
-            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            float top = -INFINITY, total = 0.f;
-            for (int i0 = 0; i0 < n; i0 += kAtOnce) {
-                float4 x[kAtOnce];
-                float m[kAtOnce], l[kAtOnce], to = top;
+        const int size = part_floats(), rows = min(kRows, a.G - row0), cap = C::kRingBytes / 4 / size;
+        int have = 0;  // 1: the sum so far lies in front
+#pragma unroll 1
+        for (int i0 = 0; i0 < n;) {
+            const int add = min(n - i0, cap - have), count = have + add;
+            const int lane = threadIdx.x & 31;
+#pragma unroll 1
+            for (int i = threadIdx.x >> 5; i < add; i += kDecWarps) {
+                const int cta = from + (i0 + i) * stride;
+                const float* const part = a.ws + decode_part_at<D, E8, NT>(cta, cta == first) + lane * 4;
+                const uint32_t dst = smem_u32(room + (have + i) * size) + lane * 16;
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const int cta = from + min(i0 + i, n - 1) * stride;
-                    const float* const part = a.ws + decode_part_at<D, E8, NT>(cta, cta == first);
-                    x[i] = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
-                    m[i] = __ldcg(part + kRows * D + r);
-                    l[i] = __ldcg(part + kRows * D + kRows + r);
+                for (int c = 0; c < kRows * (D / 4); c += 32)  // the rows that exist, then maxima and sums
+                    if (c < rows * (D / 4)) cp_async16(dst + c * 16, part + c * 4);
+                if (lane < 2 * kRows / 4) cp_async16(dst + (size - 2 * kRows) * 4, part + kRows * D);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncthreads();
+            i0 += add;
+            const float* const m = room + size - 2 * kRows;  // of the first part
+#pragma unroll 1
+            for (int e = threadIdx.x; e < rows * (D / 4); e += kDecThreads) {
+                const int r = e / (D / 4);
+                float top = -INFINITY, total = 0.f;
+#pragma unroll 4
+                for (int i = 0; i < count; ++i) top = fmaxf(top, m[i * size + r]);
+                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                for (int i = 0; i < count; ++i) {
+                    const float w = m[i * size + r] == -INFINITY ? 0.f : ex2(m[i * size + r] - top);
+                    const float4 x = *reinterpret_cast<const float4*>(room + i * size + e * 4);
+                    z = make_float4(fmaf(x.x, w, z.x), fmaf(x.y, w, z.y), fmaf(x.z, w, z.z), fmaf(x.w, w, z.w));
+                    total = fmaf(m[i * size + kRows + r], w, total);
                 }
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) to = fmaxf(to, m[i]);
-                const float f = top == -INFINITY ? 0.f : exp2f(top - to);
-                z = make_float4(z.x * f, z.y * f, z.z * f, z.w * f);
-                total *= f;
-#pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
-                    if (i0 + i < n) {
-                        const float w = m[i] == -INFINITY ? 0.f : exp2f(m[i] - to);
-                        z = make_float4(z.x + x[i].x * w, z.y + x[i].y * w, z.z + x[i].z * w, z.w + x[i].w * w);
-                        total += l[i] * w;
-                    }
-                top = to;
+                if (i0 < n) {
+                    *reinterpret_cast<float4*>(room + e * 4) = z;  // (what only this thread has read)
+                } else if (out != nullptr) {
+                    *reinterpret_cast<float4*>(out + e * 4) = z;
+                } else {
+                    const float inv = 1.f / total;
+                    T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + e % (D / 4) * 4;
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+                }
             }
-            if (out != nullptr) {
-                // (in place of the part that this very thread has read; its maximum and sum are still read by others)
-                *reinterpret_cast<float4*>(out + r * D + d) = z;
-            } else {
-                T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
-                const float inv = 1.f / total;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+            if (i0 >= n && out == nullptr) break;
+            // maximum and sum of the rows, once all have read the old ones
+            float top = -INFINITY, total = 0.f;
+            const int r = threadIdx.x;
+            if (r < rows) {
+                for (int i = 0; i < count; ++i) top = fmaxf(top, m[i * size + r]);
+                for (int i = 0; i < count; ++i)
+                    total = fmaf(m[i * size + kRows + r], m[i * size + r] == -INFINITY ? 0.f : ex2(m[i * size + r] - top), total);
             }
-            if (d == 0) {
-                scratch[r] = top;
-                scratch[kRows + r] = total;
+            __syncthreads();
+            if (r < rows) {
+                float* const to = i0 < n ? room + size - 2 * kRows : out + kRows * D;
+                to[r] = top;
+                to[kRows + r] = total;
             }
+            have = 1;
+            __syncthreads();
         }
-        if (out == nullptr) return;
-        __syncthreads();
-        if (threadIdx.x < kRows && row0 + threadIdx.x < a.G) {
-            out[kRows * D + threadIdx.x] = scratch[threadIdx.x];
-            out[kRows * D + kRows + threadIdx.x] = scratch[kRows + threadIdx.x];
-        }
+        __syncthreads();  // (the ring is free again)
     }
     // All threads, once: this CTA's parts are in their places (`dead`: they never will be; only the counts have to go on).
     __device__ __forceinline__ void parts_done(const DecodeBroken (&item)[2], bool dead) const {
-        const int cta = blockIdx.x;
-        __threadfence();  // the parts are visible before they count
+        const int cta = blockIdx.x, group = join_group();
         __syncthreads();
         if (threadIdx.x == 0 || threadIdx.x == 32) {  // (a lane of its own for each: the two round trips overlap)
+            __threadfence();  // the CTA's parts are visible before they count
             const DecodeBroken& it = item[threadIdx.x / 32];
             bool all = false;
             if (it.first >= 0) {
-                const int from = it.first + (cta - it.first) / kJoin * kJoin, n = min(kJoin, it.last - from + 1);
+                const int from = it.first + (cta - it.first) / group * group, n = min(group, it.last - from + 1);
                 all = n == 1 || count_up(from, from == it.first ? 8 : 0, n);
             }
             __threadfence();
             s_flag[threadIdx.x / 32] = all;
         }
         __syncthreads();
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 2; ++k) {
-            const DecodeBroken& it = item[k];
             if (s_flag[k] == 0) continue;
-            const int groups = (it.last - it.first) / kJoin + 1, from = it.first + (cta - it.first) / kJoin * kJoin;
-            const int n = min(kJoin, it.last - from + 1), row0 = (it.hk - it.h * a.row_blocks) * kRows;
-            float* const place = groups == 1 ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == it.first);
-            if (n > 1 && !dead) sum(it.first, from, 1, n, place, it.b, it.h, row0);
-            if (groups == 1) continue;
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                s_flag[k] = count_up(it.first, 16, groups);
-                __threadfence();
+            const DecodeBroken it = k == 0 ? item[0] : item[1];
+            const int groups = (it.last - it.first) / group + 1, row0 = (it.hk - it.h * a.row_blocks) * kRows;
+            int from = it.first + (cta - it.first) / group * group, stride = 1, n = min(group, it.last - from + 1);
+            bool final = groups == 1;
+#pragma unroll 1
+            for (;;) {
+                float* const place = final ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == it.first);
+                if (n > 1 && !dead) sum(it.first, from, stride, n, place, it.b, it.h, row0);
+                if (final) break;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    __threadfence();
+                    s_flag[k] = count_up(it.first, 16, groups);
+                    __threadfence();
+                }
+                __syncthreads();
+                if (s_flag[k] == 0) break;
+                from = it.first;
+                stride = group;
+                n = groups;
+                final = true;
             }
-            __syncthreads();
-            if (s_flag[k] != 0 && !dead) sum(it.first, it.first, kJoin, groups, nullptr, it.b, it.h, row0);
         }
     }
 };
@@ -371,8 +417,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     if (tid == 0) s_dead = *reinterpret_cast<volatile int*>(a.status);  // (one reading for the whole CTA)
 
     // ---- this CTA's piece of the line of units; each warp finds it for itself
+    // (in the line an item is its units behind kItemCost places that stand for its own cost)
     unsigned int u0, u1, piece;
-    DecodeCursor cc;
+    DecodeCursor<C::kItemCost> cc;
     {
         const int per_lane = (a.B + 31) / 32, b_lo = lane * per_lane;
         unsigned int mine = 0, rows_at_all = 0;
@@ -380,7 +427,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             const int n = __ldg(a.lengths + b);
             if (n > a.c.capacity) report(a.status, kStatusBadLength);
             if (a.cos != nullptr && n > a.n_pos) report(a.status, kStatusBadPosition);
-            mine += units_of(min(max(n, 0), a.c.capacity));
+            if (n > 0) mine += units_of(min(n, a.c.capacity)) + C::kItemCost;
             rows_at_all += n > 0;
         }
         unsigned int before = mine;  // inclusive sums
@@ -391,7 +438,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         }
         const unsigned int sum = __shfl_sync(0xffffffffu, before, 31), total = sum * HK;  // (the host has seen to it that this fits)
         const unsigned int average = sum / max(__reduce_add_sync(0xffffffffu, rows_at_all), 1u);
-        piece = max((total + n_ctas - 1) / n_ctas, min(static_cast<unsigned int>(kDecMinUnits), max(average, 1u)));
+        piece = max((total + n_ctas - 1) / n_ctas, min(static_cast<unsigned int>(kDecMinUnits + C::kItemCost), max(average, 1u)));
         u0 = piece * blockIdx.x;
         u1 = min(u0 + piece, total);
         before -= mine;
@@ -399,7 +446,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         int b = b_lo;
         if (here >> lane & 1) {
             for (;;) {
-                const unsigned int n = units_of(cached_rows(a, b));
+                const int rows = cached_rows(a, b);
+                const unsigned int n = rows > 0 ? units_of(rows) + C::kItemCost : 0;
                 if (u0 < (before + n) * HK) break;
                 before += n;
                 ++b;
@@ -412,10 +460,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         if (here != 0) {
             cc.len = cached_rows(a, cc.b);
             cc.nt = units_of(cc.len);
-            cc.hk = in_b / cc.nt;
-            cc.t = in_b - cc.hk * cc.nt;
+            cc.hk = in_b / (cc.nt + C::kItemCost);
+            cc.t = static_cast<int>(in_b - cc.hk * (cc.nt + C::kItemCost)) - C::kItemCost;
             cc.h = cc.hk / a.row_blocks;
             cc.left = u1 - u0;
+            if (cc.t < 0) {  // in front of the item's first unit
+                cc.left += cc.t;
+                cc.t = 0;
+            }
         }
     }
     auto empty_rows = [&] {  // sequences without rows have no units: their output is zero
@@ -425,16 +477,16 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                     reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
                         make_uint4(0, 0, 0, 0);
     };
-    if (cc.left == 0) {  // (all warps of the CTA alike)
+    if (cc.left <= 0) {  // (all warps of the CTA alike)
         __syncthreads();
         if (s_dead == 0) empty_rows();
         return;
     }
     // the broken items: the one that began before this piece (or fills it), and the one that begins in it and goes on
     DecodeBroken broken[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};
-    if (cc.t > 0) broken[0] = {static_cast<int>((u0 - cc.t) / piece), static_cast<int>((u0 - cc.t + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
+    if (cc.t > 0) broken[0] = {static_cast<int>((u1 - cc.left - cc.t) / piece), static_cast<int>((u1 - cc.left - cc.t + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
     auto begins_and_goes_on = [&](int n) {  // n units of item cc are here
-        if (cc.t == 0 && n < cc.nt) broken[1] = {static_cast<int>(blockIdx.x), static_cast<int>((u1 - 1 + (cc.nt - n)) / piece), cc.b, cc.hk, cc.h};
+        if (cc.t == 0 && n < cc.nt) broken[1] = {static_cast<int>(blockIdx.x), static_cast<int>((u1 - cc.left + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
     };
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
@@ -455,14 +507,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     typename R::Words gamma;
     if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, lane);
 
-    DecodeCursor pc = cc;
+    auto pc = cc;
     int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
     int page = 0, row0_in_page = 0;              // of the unit that is being copied
-    bool fresh = true;                           // the producer stands at an item whose pages it has not looked up
     constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kCopies = kDecKeys / kRowsAtOnce;
     const int piece16 = lane % kPieces, r_lane = lane / kPieces;
     const uint32_t dst_lane = ring + r_lane * C::kRowBytes + ((piece16 ^ (r_lane & 7)) << 4);
     // 16 rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
+    const uint64_t policy = evict_first_policy();
     auto copy_rows = [&](int slot, const unsigned char* pool, long long sp, long long sh, long long ss, const unsigned char* scale,
                          long long scale_sp, long long scale_sh) {
         int n = pc.len - (pc.t * kDecUnit + warp * kDecKeys);
@@ -475,37 +527,37 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         };
         if (n >= kDecKeys && ss == C::kRowBytes) {
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) cp_async16(dst(i), src + i * kRowsAtOnce * C::kRowBytes);
+            for (int i = 0; i < kCopies; ++i) cp_async16(dst(i), src + i * kRowsAtOnce * C::kRowBytes, policy);
         } else {
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < kCopies; ++i) {
                 const bool take = r_lane + i * kRowsAtOnce < n;
-                cp_async16(dst(i), src + (take ? i * kRowsAtOnce * ss : 0), take);
+                cp_async16_or_zero(dst(i), src + (take ? i * kRowsAtOnce * ss : 0), take);
             }
         }
         if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
-            if (lane == 0) cp_async16(smem_u32(scales) + slot * kDecKeys, scale + page * scale_sp + pc.h * scale_sh + row0_in_page);
+            if (lane == 0) cp_async16(smem_u32(scales) + slot * kDecKeys, scale + page * scale_sp + pc.h * scale_sh + row0_in_page, policy);
+        }
+    };
+    // pages of the units from pc.t on; looked at when the next K rows are asked for
+    auto look_up = [&] {
+        table_at = pc.t;
+        my_page = my_row = 0;
+        const int key = (pc.t + lane) * kDecUnit + warp * kDecKeys;
+        if (pc.t + lane < pc.nt && key < pc.len) {
+            const int i = key / a.c.page_size;
+            my_row = key - i * a.c.page_size;
+            my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
         }
     };
     auto issue_k = [&](int slot) {
         if (pc.left > 0) {
-            if (fresh || pc.t - table_at >= 32) {
-                fresh = false;
-                table_at = pc.t;
-                const int key = (pc.t + lane) * kDecUnit + warp * kDecKeys;
-                my_page = my_row = 0;
-                if (pc.t + lane < pc.nt && key < pc.len) {
-                    const int i = key / a.c.page_size;
-                    my_row = key - i * a.c.page_size;
-                    my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
-                    if (static_cast<unsigned>(my_page) >= static_cast<unsigned>(a.c.n_pages)) {
-                        report(a.status, kStatusBadPage);
-                        my_page = -1;  // (nothing is copied: the keys are whatever the slot held)
-                    }
-                }
-            }
             page = __shfl_sync(0xffffffffu, my_page, pc.t - table_at);
             row0_in_page = __shfl_sync(0xffffffffu, my_row, pc.t - table_at);
+            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
+                if (lane == 0) report(a.status, kStatusBadPage);
+                page = -1;  // (nothing is copied: the keys are whatever the slot held)
+            }
             copy_rows(slot, a.c.k, a.c.k_sp, a.c.k_sh, a.c.k_ss, a.c.k_scale, a.c.ks_sp, a.c.ks_sh);
         }
         cp_async_commit();
@@ -517,11 +569,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             --pc.left;
             if (pc.t == pc.nt && pc.left > 0) {
                 pc.next_item(a, HK);
-                fresh = true;
+                if (pc.left > 0) look_up();
+            } else if (pc.t - table_at == 32) {
+                look_up();
             }
         }
         cp_async_commit();
     };
+    look_up();
 #pragma unroll 1
     for (int s = 0; s < C::kSlots - 1; s += 2) {
         issue_k(s);
@@ -623,13 +678,11 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         const int n = min(cc.nt - cc.t, cc.left);
         if (n <= 0) break;
         const int h = cc.h, row0 = (cc.hk - h * a.row_blocks) * kRows;
-        DecodeCursor nc = cc;  // the item after this one: its query rows are on their way meanwhile
+        auto nc = cc;  // the item after this one: its query rows are on their way meanwhile
         nc.t += n;
         nc.left -= n;
-        if (nc.left > 0) {
-            nc.next_item(a, HK);
-            rows.load(a, nc);
-        }
+        if (nc.left > 0) nc.next_item(a, HK);
+        if (nc.left > 0) rows.load(a, nc);
         uint4 qf[C::kQueryInRegs ? NT : 1][C::kQueryInRegs ? kDT : 1];
         if constexpr (C::kQueryInRegs) {
 #pragma unroll
@@ -839,7 +892,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 float top = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, merge_m[w * kRows + u * 8 + 2 * t4 + c]);
-                const float f = mv[u][c] == -INFINITY ? 0.f : exp2f(mv[u][c] - (top == -INFINITY ? 0.f : top));
+                const float f = mv[u][c] == -INFINITY ? 0.f : ex2(mv[u][c] - (top == -INFINITY ? 0.f : top));
                 // (a warp without keys has a zero output; one whose scores are all -inf keeps a NaN that it may hold)
 #pragma unroll
                 for (int i = 0; i < kDT; ++i) {
@@ -880,7 +933,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
 #pragma unroll
                     for (int w = 0; w < kDecWarps; ++w) {
                         const float lw = merge_l[w * kRows + r];
-                        sum += lw == 0.f ? 0.f : lw * exp2f(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
+                        sum += lw == 0.f ? 0.f : lw * ex2(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
                     }
                     if (whole) {
                         T* const dst = reinterpret_cast<T*>(a.out) + cc.b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
@@ -898,7 +951,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             }
         cc = nc;
     }
-    cp_async_wait<0>();  // (the ring's first bytes serve the joins)
+    cp_async_wait<0>();  // (the ring serves the joins)
     DecodeJoin<D, T, E8, NT>{a, reinterpret_cast<float*>(smem), s_flag}.parts_done(broken, false);
 }
 

@@ -139,11 +139,11 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     kf::DecodeArgs args = a;
     args.row_blocks = (a.G + 8 * NT - 1) / (8 * NT);
     // no more CTAs than the batch can have pieces of work
-    const long long most = static_cast<long long>(a.B) * a.Hkv * args.row_blocks *
-                           ((a.c.capacity + kf::kDecUnit - 1) / kf::kDecUnit);
+    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, per_item = (a.c.capacity + kf::kDecUnit - 1) / kf::kDecUnit;
+    const long long most = items * (per_item + kf::DecodeCfg<D, E8, NT>::kItemCost);
     if (most > 0x7fffffffLL) return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
     const long long fit = decode_ctas<D, E8, NT>();
-    const unsigned grid = (unsigned)(most < fit ? most : fit);
+    const unsigned grid = (unsigned)(items * per_item < fit ? items * per_item : fit);
     if (grid > 1) {
         if (int r = join_words(st, &args.arrived)) return r;
         if (args.arrived == nullptr) {  // then words in the workspace, cleared by the graph itself
