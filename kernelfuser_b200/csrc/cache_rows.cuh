@@ -22,14 +22,15 @@ constexpr int kStatusBadPosition = 913;  // a position behind the last row of th
 struct CacheView {
     unsigned char *k, *v;                        // [n_pages, H, page_size, D]; strides in BYTES
     unsigned char *k_scale, *v_scale;            // [n_pages, H, page_size] exponent bytes (8-bit cache)
-    long long k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;
-    long long ks_sp, ks_sh, vs_sp, vs_sh;
+    int k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;      // (a page's place: a 32 x 32 -> 64 bit product)
+    int ks_sp, ks_sh, vs_sp, vs_sh;
     const int* pages;                            // [B, max_pages]
     long long pages_sb;
     int n_pages, page_size, max_pages;
     int capacity;                                // max_pages * page_size, at most 2^31 - 1
 };
 
+__device__ __forceinline__ long long wide(int a, int b) { return static_cast<long long>(a) * b; }
 __device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
 
 // Two floats to two e4m3 (in the low 16 bits, `lo` first), to nearest even; values above 448 saturate.
@@ -227,8 +228,8 @@ __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendA
     const int h0 = blockIdx.y * a.heads_per_group, h1 = min(h0 + a.heads_per_group, a.H);
     const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + s * a.k_ss;
     const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + s * a.v_ss;
-    unsigned char* kd = a.c.k + page * a.c.k_sp + row * a.c.k_ss;
-    unsigned char* vd = a.c.v + page * a.c.v_sp + row * a.c.v_ss;
+    unsigned char* kd = a.c.k + wide(page, a.c.k_sp) + wide(row, a.c.k_ss);
+    unsigned char* vd = a.c.v + wide(page, a.c.v_sp) + wide(row, a.c.v_ss);
     for (int h = h0; h < h1; ++h) {
         typename R::Words kw = {}, vw = {};
         if (valid) {
@@ -245,11 +246,11 @@ __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendA
                 if (valid) *reinterpret_cast<decltype(value)*>(dst + at) = value;
             };
         };
-        const uint32_t ke = k.template store<T, E8>(sub, to(kd + h * a.c.k_sh));
-        const uint32_t ve = v.template store<T, E8>(sub, to(vd + h * a.c.v_sh));
+        const uint32_t ke = k.template store<T, E8>(sub, to(kd + wide(h, a.c.k_sh)));
+        const uint32_t ve = v.template store<T, E8>(sub, to(vd + wide(h, a.c.v_sh)));
         if (E8 && valid && sub == 0) {
-            a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + row] = static_cast<unsigned char>(ke);
-            a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + row] = static_cast<unsigned char>(ve);
+            a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row] = static_cast<unsigned char>(ke);
+            a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row] = static_cast<unsigned char>(ve);
         }
     }
 }
@@ -292,8 +293,8 @@ __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs 
                 report(a.status, kStatusBadPage);
                 continue;
             }
-            const unsigned char* kp = a.c.k + page * a.c.k_sp + h * a.c.k_sh + row * a.c.k_ss;
-            const unsigned char* vp = a.c.v + page * a.c.v_sp + h * a.c.v_sh + row * a.c.v_ss;
+            const unsigned char* kp = a.c.k + wide(page, a.c.k_sp) + wide(h, a.c.k_sh) + wide(row, a.c.k_ss);
+            const unsigned char* vp = a.c.v + wide(page, a.c.v_sp) + wide(h, a.c.v_sh) + wide(row, a.c.v_ss);
             if constexpr (E8) {
                 const uint2 k2 = __ldcs(reinterpret_cast<const uint2*>(kp) + sub);
                 const uint2 v2 = __ldcs(reinterpret_cast<const uint2*>(vp) + sub);
@@ -301,8 +302,8 @@ __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs 
                 kx[u].y = k2.y;
                 vx[u].x = v2.x;
                 vx[u].y = v2.y;
-                kf[u] = scale_value(a.c.k_scale[page * a.c.ks_sp + h * a.c.ks_sh + row]);
-                vf[u] = scale_value(a.c.v_scale[page * a.c.vs_sp + h * a.c.vs_sh + row]);
+                kf[u] = scale_value(a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row]);
+                vf[u] = scale_value(a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row]);
             } else {
                 kx[u] = __ldcs(reinterpret_cast<const uint4*>(kp) + sub);
                 vx[u] = __ldcs(reinterpret_cast<const uint4*>(vp) + sub);

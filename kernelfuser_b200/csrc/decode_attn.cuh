@@ -6,7 +6,7 @@
 // What bounds it.  Every cached byte is read once and serves G query heads: 4 D G operations per 4 D bytes of a 16-bit
 // cache, a few operations a byte, so HBM sets the time and everything else has to stay out of its way.
 //
-// Work split.  The unit of work is 64 keys of one (sequence, KV head).  All units of the launch are laid in one line and
+// Work split.  The unit of work is 64 keys of one (sequence, KV head), or 128 of an 8-bit cache.  All units of the launch are laid in one line and
 // every CTA takes an equal piece of it, found from the lengths on the device: ragged batches and single long sequences
 // load all SMs alike, and a captured launch follows its lengths.  A CTA's piece covers whole (sequence, head) items and
 // at most two broken ones; a broken item's parts meet in the workspace, where the CTA that comes last joins them, in the
@@ -31,6 +31,7 @@
 // whose base for O is kept apart from the one for the sum.
 #pragma once
 #include <type_traits>
+#include <utility>
 
 #include "cache_rows.cuh"
 
@@ -53,29 +54,30 @@ struct DecodeArgs {
 };
 
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
-constexpr int kDecKeys = 16;                    // keys of a warp's step
-constexpr int kDecUnit = kDecKeys * kDecWarps;  // keys of a unit
 // A CTA's piece is at least this many units, or the average item: a join costs about as much as four units of one warp each.
-constexpr int kDecMinUnits = 4;
+#ifndef KF_MINU
+#define KF_MINU 4
+#endif
+constexpr int kDecMinUnits = KF_MINU;
 
-#ifndef KF_E8_CTAS
-#define KF_E8_CTAS 3
-#define KF_E8_SLOTS 7
-#endif
-#ifndef KF_ITEM_COST
-#define KF_ITEM_COST 1
-#endif
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kItemCost = KF_ITEM_COST;
+    static constexpr int kTiles = E8 ? 2 : 1, kKeys = 16 * kTiles, kUnit = kKeys * kDecWarps;  // keys of a warp's step, of a unit
     static constexpr int kRowBytes = D * (E8 ? 1 : 2);
-    static constexpr int kSlotBytes = kDecKeys * kRowBytes;           // K or V rows of a step
-    static constexpr int kScaleBytes = E8 ? kDecKeys : 0;             // and their scales
+    // What an item costs beside its units, in units of its keys: about 3 us of a CTA (looking up its rows, preparing its
+    // queries, meeting of the warps), which hold a unit of 64 KB or two of 32.  32 ragged sequences of up to 1500 rows: 1 -> 36
+    // us, 2 -> 28.7, 3 -> 27.7; wide heads 16 x 2047: 34.7, 32.8, 33.4; uniform batches do not care.
+    static constexpr int kItemCost = kRowBytes == 512 ? 2 : 3;
+    static constexpr int kSlotBytes = kKeys * kRowBytes;              // K or V rows of a step
+    static constexpr int kScaleBytes = E8 ? kKeys : 0;                // and their scales
     static constexpr bool kQueryInRegs = D * NT <= 256;               // else its fragments are read for every step
-    static constexpr int kCtasPerSm = E8 && D == 128 && NT == 1 ? KF_E8_CTAS : kQueryInRegs ? 2 : 1;
-    // slots of a warp's ring: 100 KB per CTA, as far as two of them fit an SM
-    static constexpr int kSlots = E8 ? (D == 128 ? (NT == 1 ? KF_E8_SLOTS : 10) : 5) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
-    static constexpr int kMergeCols = D == 256 && !E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
+    static constexpr int kCtasPerSm = E8 && D == 128 && NT == 1 ? 3 : kQueryInRegs ? 2 : 1;
+    // An 8-bit cache is bound by the instructions that widen it as much as by HBM: steps of 32 keys share what a step costs
+    // and have twice as many independent products (64 sequences of 4096 rows, G = 4: 118 -> 98 us, floor 83), and three CTAs
+    // give the schedulers a third warp each (135 -> 116 us with steps of 16; four, at 128 registers: 124).
+    // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
+    static constexpr int kSlots = E8 ? (D == 128 ? (NT == 1 ? 3 : 5) : 3) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
+    static constexpr int kMergeCols = D == 256 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
     static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
@@ -100,8 +102,12 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+template <int DST, int SRC> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "l"(policy), "n"(DST), "n"(SRC)
+                 : "memory");
+}
+template <typename F, int... I> __device__ __forceinline__ void each_index(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -139,10 +145,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ int cached_rows(const DecodeArgs& a, int b) { return min(max(__ldg(a.lengths + b), 0), a.c.capacity); }
-__device__ __forceinline__ int units_of(int len) { return (len + kDecUnit - 1) / kDecUnit; }
+template <int UNIT> __device__ __forceinline__ int units_of(int len) { return (len + UNIT - 1) / UNIT; }
 
 // A place in the line of units: unit t of nt of item hk of sequence b.
-template <int COST> struct DecodeCursor {
+template <int UNIT, int COST> struct DecodeCursor {
     int b, hk, h, t, nt, len;
     int left;  // of the line up to the end of the CTA's piece
     // to the next item, if the piece reaches it
@@ -155,7 +161,7 @@ template <int COST> struct DecodeCursor {
         if (hk < HK) return;
         hk = h = 0;
         do len = cached_rows(a, ++b); while (len == 0 && b + 1 < a.B);
-        nt = units_of(len);
+        nt = units_of<UNIT>(len);
     }
 };
 
@@ -419,7 +425,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     // ---- this CTA's piece of the line of units; each warp finds it for itself
     // (in the line an item is its units behind kItemCost places that stand for its own cost)
     unsigned int u0, u1, piece;
-    DecodeCursor<C::kItemCost> cc;
+    DecodeCursor<C::kUnit, C::kItemCost> cc;
     {
         const int per_lane = (a.B + 31) / 32, b_lo = lane * per_lane;
         unsigned int mine = 0, rows_at_all = 0;
@@ -427,7 +433,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             const int n = __ldg(a.lengths + b);
             if (n > a.c.capacity) report(a.status, kStatusBadLength);
             if (a.cos != nullptr && n > a.n_pos) report(a.status, kStatusBadPosition);
-            if (n > 0) mine += units_of(min(n, a.c.capacity)) + C::kItemCost;
+            if (n > 0) mine += units_of<C::kUnit>(min(n, a.c.capacity)) + C::kItemCost;
             rows_at_all += n > 0;
         }
         unsigned int before = mine;  // inclusive sums
@@ -447,7 +453,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         if (here >> lane & 1) {
             for (;;) {
                 const int rows = cached_rows(a, b);
-                const unsigned int n = rows > 0 ? units_of(rows) + C::kItemCost : 0;
+                const unsigned int n = rows > 0 ? units_of<C::kUnit>(rows) + C::kItemCost : 0;
                 if (u0 < (before + n) * HK) break;
                 before += n;
                 ++b;
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         cc.left = 0;
         if (here != 0) {
             cc.len = cached_rows(a, cc.b);
-            cc.nt = units_of(cc.len);
+            cc.nt = units_of<C::kUnit>(cc.len);
             cc.hk = in_b / (cc.nt + C::kItemCost);
             cc.t = static_cast<int>(in_b - cc.hk * (cc.nt + C::kItemCost)) - C::kItemCost;
             cc.h = cc.hk / a.row_blocks;
@@ -508,43 +514,59 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, lane);
 
     auto pc = cc;
-    int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's keys of unit table_at + i
-    int page = 0, row0_in_page = 0;              // of the unit that is being copied
-    constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kCopies = kDecKeys / kRowsAtOnce;
+    constexpr int kLook = 32 / C::kTiles;        // units whose pages the lanes hold
+    int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's 16 keys i of the units from table_at on
+    int page[C::kTiles] = {}, page_row[C::kTiles] = {};  // of the unit that is being copied
+    constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kCopies = 16 / kRowsAtOnce;
     const int piece16 = lane % kPieces, r_lane = lane / kPieces;
     const uint32_t dst_lane = ring + r_lane * C::kRowBytes + ((piece16 ^ (r_lane & 7)) << 4);
-    // 16 rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
     const uint64_t policy = evict_first_policy();
-    auto copy_rows = [&](int slot, const unsigned char* pool, long long sp, long long sh, long long ss, const unsigned char* scale,
-                         long long scale_sp, long long scale_sh) {
-        int n = pc.len - (pc.t * kDecUnit + warp * kDecKeys);
-        if (n <= 0 || page < 0) return;
-        n -= a.new_k != nullptr;  // (the last row is not in the cache yet)
-        const unsigned char* const src = pool + page * sp + pc.h * sh + (row0_in_page + r_lane) * ss + piece16 * 16;
-        const uint32_t base = dst_lane + slot * C::kSlotBytes;
-        auto dst = [&](int i) {  // row r_lane + i * kRowsAtOnce (r_lane is below kRowsAtOnce, a power of two)
-            return (base ^ ((i * kRowsAtOnce & 7) << 4)) + i * kRowsAtOnce * C::kRowBytes;
-        };
-        if (n >= kDecKeys && ss == C::kRowBytes) {
-#pragma unroll
-            for (int i = 0; i < kCopies; ++i) cp_async16(dst(i), src + i * kRowsAtOnce * C::kRowBytes, policy);
-        } else {
-#pragma unroll 1
-            for (int i = 0; i < kCopies; ++i) {
-                const bool take = r_lane + i * kRowsAtOnce < n;
-                cp_async16_or_zero(dst(i), src + (take ? i * kRowsAtOnce * ss : 0), take);
-            }
+    // this lane's place in row 0 of page 0 of the item's head, and the scales of that row
+    const unsigned char *k_src = nullptr, *v_src = nullptr, *ks_src = nullptr, *vs_src = nullptr;
+    auto head_sources = [&] {
+        k_src = a.c.k + wide(pc.h, a.c.k_sh) + wide(r_lane, a.c.k_ss) + piece16 * 16;
+        v_src = a.c.v + wide(pc.h, a.c.v_sh) + wide(r_lane, a.c.v_ss) + piece16 * 16;
+        if constexpr (E8) {
+            ks_src = a.c.k_scale + wide(pc.h, a.c.ks_sh);
+            vs_src = a.c.v_scale + wide(pc.h, a.c.vs_sh);
         }
-        if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
-            if (lane == 0) cp_async16(smem_u32(scales) + slot * kDecKeys, scale + page * scale_sp + pc.h * scale_sh + row0_in_page, policy);
+    };
+    // a step's rows of the pool to a slot; rows behind the sequence become zeros, whatever the page holds there
+    auto copy_rows = [&](int slot, const unsigned char* pool, int sp, int ss, const unsigned char* scale, int scale_sp) {
+        int n = pc.len - (pc.t * C::kUnit + warp * C::kKeys);
+        if (n <= 0) return;
+        n -= a.new_k != nullptr;  // (the last row is not in the cache yet)
+#pragma unroll
+        for (int tile = 0; tile < C::kTiles; ++tile) {
+            const unsigned char* const src = pool + wide(page[tile], sp) + wide(page_row[tile], ss);
+            const uint32_t base = dst_lane + slot * C::kSlotBytes + tile * 16 * C::kRowBytes;
+            auto dst = [&](int i) {  // row r_lane + i * kRowsAtOnce (r_lane is below kRowsAtOnce, a power of two)
+                return (base ^ ((i * kRowsAtOnce & 7) << 4)) + i * kRowsAtOnce * C::kRowBytes;
+            };
+            if (n >= 16 * (tile + 1) && ss == C::kRowBytes) {
+                each_index([&](auto i) {
+                    constexpr int kI = decltype(i)::value, kStep = kI * kRowsAtOnce * C::kRowBytes;
+                    cp_async16<kStep, kStep>(base ^ ((kI * kRowsAtOnce & 7) << 4), src, policy);
+                }, std::make_integer_sequence<int, kCopies>{});
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < kCopies; ++i) {
+                    const bool take = r_lane + i * kRowsAtOnce < n - 16 * tile;
+                    cp_async16_or_zero(dst(i), src + (take ? wide(i * kRowsAtOnce, ss) : 0), take);
+                }
+            }
+            if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
+                if (lane == 0)
+                    cp_async16<0, 0>(smem_u32(scales) + slot * C::kKeys + 16 * tile, scale + wide(page[tile], scale_sp) + page_row[tile], policy);
+            }
         }
     };
     // pages of the units from pc.t on; looked at when the next K rows are asked for
     auto look_up = [&] {
         table_at = pc.t;
         my_page = my_row = 0;
-        const int key = (pc.t + lane) * kDecUnit + warp * kDecKeys;
-        if (pc.t + lane < pc.nt && key < pc.len) {
+        const int unit = pc.t + lane / C::kTiles, key = unit * C::kUnit + warp * C::kKeys + lane % C::kTiles * 16;
+        if (unit < pc.nt && key < pc.len) {
             const int i = key / a.c.page_size;
             my_row = key - i * a.c.page_size;
             my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
@@ -552,30 +574,37 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     };
     auto issue_k = [&](int slot) {
         if (pc.left > 0) {
-            page = __shfl_sync(0xffffffffu, my_page, pc.t - table_at);
-            row0_in_page = __shfl_sync(0xffffffffu, my_row, pc.t - table_at);
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
-                if (lane == 0) report(a.status, kStatusBadPage);
-                page = -1;  // (nothing is copied: the keys are whatever the slot held)
+#pragma unroll
+            for (int tile = 0; tile < C::kTiles; ++tile) {
+                page[tile] = __shfl_sync(0xffffffffu, my_page, (pc.t - table_at) * C::kTiles + tile);
+                page_row[tile] = __shfl_sync(0xffffffffu, my_row, (pc.t - table_at) * C::kTiles + tile);
+                if (static_cast<unsigned>(page[tile]) >= static_cast<unsigned>(a.c.n_pages)) {
+                    if (lane == 0) report(a.status, kStatusBadPage);
+                    page[tile] = 0;  // (what the call gives is not to be trusted then)
+                }
             }
-            copy_rows(slot, a.c.k, a.c.k_sp, a.c.k_sh, a.c.k_ss, a.c.k_scale, a.c.ks_sp, a.c.ks_sh);
+            copy_rows(slot, k_src, a.c.k_sp, a.c.k_ss, ks_src, a.c.ks_sp);
         }
         cp_async_commit();
     };
     auto issue_v = [&](int slot) {
         if (pc.left > 0) {
-            copy_rows(slot, a.c.v, a.c.v_sp, a.c.v_sh, a.c.v_ss, a.c.v_scale, a.c.vs_sp, a.c.vs_sh);
+            copy_rows(slot, v_src, a.c.v_sp, a.c.v_ss, vs_src, a.c.vs_sp);
             ++pc.t;
             --pc.left;
             if (pc.t == pc.nt && pc.left > 0) {
                 pc.next_item(a, HK);
-                if (pc.left > 0) look_up();
-            } else if (pc.t - table_at == 32) {
+                if (pc.left > 0) {
+                    head_sources();
+                    look_up();
+                }
+            } else if (pc.t - table_at == kLook) {
                 look_up();
             }
         }
         cp_async_commit();
     };
+    head_sources();
     look_up();
 #pragma unroll 1
     for (int s = 0; s < C::kSlots - 1; s += 2) {
@@ -639,22 +668,22 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 if (write) *reinterpret_cast<decltype(value)*>(pool + at) = value;
             };
         };
-        const long long p = write ? pg : 0;
-        new_ke = k.template store<T, E8>(lane, to(new_rows, a.c.k + p * a.c.k_sp + cc.h * a.c.k_sh + row * a.c.k_ss));
-        new_ve = v.template store<T, E8>(lane, to(new_rows + C::kRowBytes, a.c.v + p * a.c.v_sp + cc.h * a.c.v_sh + row * a.c.v_ss));
+        const int p = write ? pg : 0;
+        new_ke = k.template store<T, E8>(lane, to(new_rows, a.c.k + wide(p, a.c.k_sp) + wide(cc.h, a.c.k_sh) + wide(row, a.c.k_ss)));
+        new_ve = v.template store<T, E8>(lane, to(new_rows + C::kRowBytes, a.c.v + wide(p, a.c.v_sp) + wide(cc.h, a.c.v_sh) + wide(row, a.c.v_ss)));
         if (E8 && write && lane == 0) {
-            a.c.k_scale[p * a.c.ks_sp + cc.h * a.c.ks_sh + row] = static_cast<unsigned char>(new_ke);
-            a.c.v_scale[p * a.c.vs_sp + cc.h * a.c.vs_sh + row] = static_cast<unsigned char>(new_ve);
+            a.c.k_scale[wide(p, a.c.ks_sp) + wide(cc.h, a.c.ks_sh) + row] = static_cast<unsigned char>(new_ke);
+            a.c.v_scale[wide(p, a.c.vs_sp) + wide(cc.h, a.c.vs_sh) + row] = static_cast<unsigned char>(new_ve);
         }
         __syncwarp();
     };
     // and from there behind the cached rows of the step in `slot`
     auto place_new = [&](int slot, int v) {
-        const int r = (cc.len - 1) % kDecKeys;
+        const int r = (cc.len - 1) % C::kKeys;
         if (lane < kPieces)
             *reinterpret_cast<uint4*>(smem + (warp * C::kSlots + slot) * C::kSlotBytes + r * C::kRowBytes + ((lane ^ (r & 7)) << 4)) =
                 *reinterpret_cast<const uint4*>(new_rows + v * C::kRowBytes + lane * 16);
-        if (E8 && lane == 0) scales[slot * kDecKeys + r] = static_cast<unsigned char>(v ? new_ve : new_ke);
+        if (E8 && lane == 0) scales[slot * C::kKeys + r] = static_cast<unsigned char>(v ? new_ve : new_ke);
         __syncwarp();
     };
 
@@ -708,62 +737,70 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             l[u][0] = l[u][1] = 0.f;
         }
         // the new token's step is the last one with keys, in the item's last unit
-        const bool has_new = a.new_k != nullptr && cc.t + n == cc.nt && warp == (cc.len - 1) % kDecUnit / kDecKeys;
+        const bool has_new = a.new_k != nullptr && cc.t + n == cc.nt && warp == (cc.len - 1) % C::kUnit / C::kKeys;
         if (has_new) prepare_new();
         for (int i_unit = 0; i_unit < n; ++i_unit) {
-            const int keys = cc.len - ((cc.t + i_unit) * kDecUnit + warp * kDecKeys);  // of the sequence, from this step's first on
+            const int keys = cc.len - ((cc.t + i_unit) * C::kUnit + warp * C::kKeys);  // of the sequence, from this step's first on
             arrive(std::false_type{});
-            float x[NT][4], w[NT][4];  // scores of keys g (0, 1), g + 8 (2, 3) and heads 2 t4, 2 t4 + 1
+            // scores of keys g (0, 1), g + 8 (2, 3) of each 16 and heads 2 t4, 2 t4 + 1
+            float x[NT][C::kTiles][4], w[NT][C::kTiles][4];
             if (has_new && i_unit == n - 1) place_new(slot, 0);
             if (keys > 0) {
-                float s[NT][2][4];  // high and low part of q': two chains of products
+                float s[NT][C::kTiles][2][4];  // high and low part of q': chains of products of their own
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[u][0][i] = s[u][1][i] = 0.f;
-                auto product = [&](int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                    for (int tile = 0; tile < C::kTiles; ++tile)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[u][tile][0][i] = s[u][tile][1][i] = 0.f;
+                auto product = [&](int tile, int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u) {
                         const uint4 f = C::kQueryInRegs ? qf[C::kQueryInRegs ? u : 0][C::kQueryInRegs ? j : 0] : frag[(u * kDT + j) * 32 + lane];
-                        mma16816<M>(s[u][0], a0, a1, a2, a3, f.x, f.y);
-                        if constexpr (kSplit) mma16816<M>(s[u][1], a0, a1, a2, a3, f.z, f.w);
+                        mma16816<M>(s[u][tile][0], a0, a1, a2, a3, f.x, f.y);
+                        if constexpr (kSplit) mma16816<M>(s[u][tile][1], a0, a1, a2, a3, f.z, f.w);
                     }
                 };
                 const uint32_t k_at = k_lane + slot * C::kSlotBytes;
 #pragma unroll
-                for (int j = 0; j < kDT; j += E8 ? 2 : 1) {
-                    uint32_t r[4];
-                    ldmatrix4(r, step32(k_at, E8 ? j / 2 : j));
-                    if constexpr (E8) {
+                for (int j = 0; j < kDT; j += E8 ? 2 : 1)
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            uint32_t a0, a1, a2, a3;
-                            widen4(r[2 * y], a0, a2);
-                            widen4(r[2 * y + 1], a1, a3);
-                            product(j + y, a0, a1, a2, a3);
+                    for (int tile = 0; tile < C::kTiles; ++tile) {
+                        uint32_t r[4];
+                        ldmatrix4(r, step32(k_at, E8 ? j / 2 : j) + tile * 16 * C::kRowBytes);
+                        if constexpr (E8) {
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                uint32_t a0, a1, a2, a3;
+                                widen4(r[2 * y], a0, a2);
+                                widen4(r[2 * y + 1], a1, a3);
+                                product(tile, j + y, a0, a1, a2, a3);
+                            }
+                        } else {
+                            product(tile, j, r[0], r[1], r[2], r[3]);
                         }
-                    } else {
-                        product(j, r[0], r[1], r[2], r[3]);
                     }
-                }
-                float f0 = 1.f, f1 = 1.f;  // scales of the keys
-                if constexpr (E8) {
-                    f0 = scale_value(scales[slot * kDecKeys + g]);
-                    f1 = scale_value(scales[slot * kDecKeys + g + 8]);
-                }
 #pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[u][i] = (kSplit ? s[u][0][i] + s[u][1][i] : s[u][0][i]) * mul[u][i & 1];
-                        if constexpr (E8) x[u][i] *= i < 2 ? f0 : f1;
+                for (int tile = 0; tile < C::kTiles; ++tile) {
+                    float f0 = 1.f, f1 = 1.f;  // scales of the keys
+                    if constexpr (E8) {
+                        f0 = scale_value(scales[slot * C::kKeys + 16 * tile + g]);
+                        f1 = scale_value(scales[slot * C::kKeys + 16 * tile + g + 8]);
                     }
-                if (keys < kDecKeys) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (g + 8 * (i >> 1) >= keys) x[u][i] = -INFINITY;
+                        for (int i = 0; i < 4; ++i) {
+                            x[u][tile][i] = (kSplit ? s[u][tile][0][i] + s[u][tile][1][i] : s[u][tile][0][i]) * mul[u][i & 1];
+                            if constexpr (E8) x[u][tile][i] *= i < 2 ? f0 : f1;
+                        }
+                }
+                if (keys < C::kKeys) {
+#pragma unroll
+                    for (int u = 0; u < NT; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4 * C::kTiles; ++i)
+                            if (g + 8 * (i >> 1) >= keys) x[u][i / 4][i % 4] = -INFINITY;
                 }
             }
             leave();
@@ -772,42 +809,48 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             if (keys > 0) {
                 bool above = false;
                 if constexpr (E8) {
-                    const uint32_t e0 = scales[slot * kDecKeys + g], e1 = scales[slot * kDecKeys + g + 8];
-                    const float ve0 = e0 == 255 ? NAN : static_cast<float>(static_cast<int>(e0) - 127);
-                    const float ve1 = e1 == 255 ? NAN : static_cast<float>(static_cast<int>(e1) - 127);
 #pragma unroll
-                    for (int u = 0; u < NT; ++u)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            w[u][i] = x[u][i] + (i < 2 ? ve0 : ve1);
-                            above |= w[u][i] > mv[u][i & 1] + kSlack;
-                        }
-                    if (keys < kDecKeys) {  // (scales behind the sequence are whatever the page holds)
+                    for (int tile = 0; tile < C::kTiles; ++tile) {
+                        const uint32_t e0 = scales[slot * C::kKeys + 16 * tile + g], e1 = scales[slot * C::kKeys + 16 * tile + g + 8];
+                        // (2^23 + e as bits: e - 127 without a conversion)
+                        const float ve0 = e0 == 255 ? NAN : __uint_as_float(0x4b000000u | e0) - 8388735.f;
+                        const float ve1 = e1 == 255 ? NAN : __uint_as_float(0x4b000000u | e1) - 8388735.f;
 #pragma unroll
                         for (int u = 0; u < NT; ++u)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (g + 8 * (i >> 1) >= keys) w[u][i] = -INFINITY;
+                            for (int i = 0; i < 4; ++i) {
+                                w[u][tile][i] = x[u][tile][i] + (i < 2 ? ve0 : ve1);
+                                above |= w[u][tile][i] > mv[u][i & 1] + kSlack;
+                            }
+                    }
+                    if (keys < C::kKeys) {  // (scales behind the sequence are whatever the page holds)
+#pragma unroll
+                        for (int u = 0; u < NT; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4 * C::kTiles; ++i)
+                                if (g + 8 * (i >> 1) >= keys) w[u][i / 4][i % 4] = -INFINITY;
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) above |= x[u][i] > m[u][i & 1] + kSlack;
+                    for (int i = 0; i < 4 * C::kTiles; ++i) above |= x[u][i / 4][i % 4] > m[u][i & 1] + kSlack;
                 if (__any_sync(0xffffffffu, above)) {  // move the bases (of the heads whose own scores ask for it) to the maxima
-                    auto top = [](float y, float z, float base) {
-                        y = fmaxf(y, z);
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-                        return y > base + kSlack ? y : base;
+                    auto top = [](const float (&y)[C::kTiles][4], int c, float base) {
+                        float z = fmaxf(y[0][c], y[0][c + 2]);
+#pragma unroll
+                        for (int tile = 1; tile < C::kTiles; ++tile) z = fmaxf(z, fmaxf(y[tile][c], y[tile][c + 2]));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 4));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 8));
+                        z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, 16));
+                        return z > base + kSlack ? z : base;
                     };
 #pragma unroll
                     for (int u = 0; u < NT; ++u)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float to = top(x[u][c], x[u][c + 2], m[u][c]);
-                            const float to_v = E8 ? top(w[u][c], w[u][c + 2], mv[u][c]) : to;
+                            const float to = top(x[u], c, m[u][c]);
+                            const float to_v = E8 ? top(w[u], c, mv[u][c]) : to;
                             l[u][c] *= m[u][c] == -INFINITY ? 0.f : ex2(m[u][c] - to);
                             const float f = mv[u][c] == -INFINITY ? 0.f : ex2(mv[u][c] - to_v);
 #pragma unroll
@@ -821,50 +864,56 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                             off_v[u][c] = to_v == -INFINITY ? 0.f : kUp - to_v;
                         }
                 }
-                uint32_t pb[NT][4];  // high and low part of the probabilities of keys 0-7, 8-15
+                uint32_t pb[NT][C::kTiles][4];  // high and low part of the probabilities of keys 0-7, 8-15
 #pragma unroll
-                for (int u = 0; u < NT; ++u) {
+                for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = ex2(x[u][i] + off[u][i & 1]);
-                        l[u][i & 1] += p;
-                        w[u][i] = E8 ? ex2(w[u][i] + off_v[u][i & 1]) : p;
+                    for (int tile = 0; tile < C::kTiles; ++tile) {
+                        float(&p)[4] = w[u][tile];
+                        uint32_t(&b)[4] = pb[u][tile];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float y = ex2(x[u][tile][i] + off[u][i & 1]);
+                            l[u][i & 1] += y;
+                            p[i] = E8 ? ex2(p[i] + off_v[u][i & 1]) : y;
+                        }
+                        if constexpr (kSplit) {
+                            split2_probabilities<M, !E8>(p[0], p[1], b[0], b[2]);
+                            split2_probabilities<M, !E8>(p[2], p[3], b[1], b[3]);
+                        } else {
+                            b[0] = Num<M>::pack(p[0], p[1]);
+                            b[1] = Num<M>::pack(p[2], p[3]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < (kSplit ? 4 : 2); ++i) b[i] = transpose8x8(b[i]);
                     }
-                    if constexpr (kSplit) {
-                        split2_probabilities<M, !E8>(w[u][0], w[u][1], pb[u][0], pb[u][2]);
-                        split2_probabilities<M, !E8>(w[u][2], w[u][3], pb[u][1], pb[u][3]);
-                    } else {
-                        pb[u][0] = Num<M>::pack(w[u][0], w[u][1]);
-                        pb[u][1] = Num<M>::pack(w[u][2], w[u][3]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < (kSplit ? 4 : 2); ++i) pb[u][i] = transpose8x8(pb[u][i]);
-                }
-                auto product = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+                auto product = [&](int tile, int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u) {
-                        mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][0], pb[u][1]);
-                        if constexpr (kSplit) mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][2], pb[u][3]);
+                        mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][tile][0], pb[u][tile][1]);
+                        if constexpr (kSplit) mma16816<M>(o[u][i], a0, a1, a2, a3, pb[u][tile][2], pb[u][tile][3]);
                     }
                 };
                 const uint32_t v_at = v_lane + slot * C::kSlotBytes;
 #pragma unroll
-                for (int i = 0; i < kDT; i += E8 ? 2 : 1) {
-                    uint32_t r[4];
-                    ldmatrix4_trans(r, step32(v_at, E8 ? i / 2 : i));
-                    if constexpr (E8) {
+                for (int tile = 0; tile < C::kTiles; ++tile)
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            // bytes {key 2t col 2g, key 2t col 2g+1, key 2t+1 col 2g, key 2t+1 col 2g+1}
-                            uint32_t a0, a1, a2, a3;
-                            widen4(__byte_perm(r[2 * y], 0, 0x3120), a0, a1);
-                            widen4(__byte_perm(r[2 * y + 1], 0, 0x3120), a2, a3);
-                            product(i + y, a0, a1, a2, a3);
+                    for (int i = 0; i < kDT; i += E8 ? 2 : 1) {
+                        uint32_t r[4];
+                        ldmatrix4_trans(r, step32(v_at, E8 ? i / 2 : i) + tile * 16 * C::kRowBytes);
+                        if constexpr (E8) {
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                // bytes {key 2t col 2g, key 2t col 2g+1, key 2t+1 col 2g, key 2t+1 col 2g+1}
+                                uint32_t a0, a1, a2, a3;
+                                widen4(__byte_perm(r[2 * y], 0, 0x3120), a0, a1);
+                                widen4(__byte_perm(r[2 * y + 1], 0, 0x3120), a2, a3);
+                                product(tile, i + y, a0, a1, a2, a3);
+                            }
+                        } else {
+                            product(tile, i, r[0], r[1], r[2], r[3]);
                         }
-                    } else {
-                        product(i, r[0], r[1], r[2], r[3]);
                     }
-                }
             }
             leave();
         }

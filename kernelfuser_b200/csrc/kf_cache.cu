@@ -53,10 +53,16 @@ int cache_view(const kf_paged_cache& c, int64_t dtype, kf::CacheView* out) {
     v.v = static_cast<unsigned char*>(c.v);
     v.k_scale = static_cast<unsigned char*>(c.k_scale);
     v.v_scale = static_cast<unsigned char*>(c.v_scale);
-    v.k_sp = c.k_stride_page * size; v.k_sh = c.k_stride_head * size; v.k_ss = c.k_stride_row * size;
-    v.v_sp = c.v_stride_page * size; v.v_sh = c.v_stride_head * size; v.v_ss = c.v_stride_row * size;
-    v.ks_sp = c.k_scale_stride_page; v.ks_sh = c.k_scale_stride_head;
-    v.vs_sp = c.v_scale_stride_page; v.vs_sh = c.v_scale_stride_head;
+    // in bytes; below 2^31 each (that of a single entry may be anything: it is never used)
+    const int64_t from[10] = {c.k_stride_page * size, c.k_stride_head * size, c.k_stride_row * size, c.v_stride_page * size,
+                              c.v_stride_head * size, c.v_stride_row * size, c.k_scale_stride_page, c.k_scale_stride_head,
+                              c.v_scale_stride_page, c.v_scale_stride_head};
+    int* const to[10] = {&v.k_sp, &v.k_sh, &v.k_ss, &v.v_sp, &v.v_sh, &v.v_ss, &v.ks_sp, &v.ks_sh, &v.vs_sp, &v.vs_sh};
+    for (int i = 0; i < 10; ++i) {
+        const bool one = extents[i < 6 ? i % 3 : i % 2] == 1, used = !one && (i < 6 || e8);
+        if (used && from[i] > 0x7fffffff) return fail(KF_EINVAL, "cache strides must be below 2^31 bytes");
+        *to[i] = used ? (int)from[i] : 0;
+    }
     v.pages = c.pages;
     v.pages_sb = c.pages_stride;
     v.n_pages = static_cast<int>(c.n_pages);
@@ -139,7 +145,7 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     kf::DecodeArgs args = a;
     args.row_blocks = (a.G + 8 * NT - 1) / (8 * NT);
     // no more CTAs than the batch can have pieces of work
-    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, per_item = (a.c.capacity + kf::kDecUnit - 1) / kf::kDecUnit;
+    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, unit = kf::DecodeCfg<D, E8, NT>::kUnit, per_item = (a.c.capacity + unit - 1) / unit;
     const long long most = items * (per_item + kf::DecodeCfg<D, E8, NT>::kItemCost);
     if (most > 0x7fffffffLL) return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
     const long long fit = decode_ctas<D, E8, NT>();
