@@ -25,7 +25,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .api import _DTYPES, _call, _major, _on_device, _raw_stream, status_word
+from .api import _DTYPES, _call, _current_device, _major, _on_device, _raw_stream, _status, status_word
 
 _CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.KF_E4M3}
 # The structs of include/kf_b200.h: 8-byte fields throughout.
@@ -55,55 +55,80 @@ class PagedCache(NamedTuple):
                            for _ in range(2)))
 
 
+_E8, _SCALE, _INT = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32
+_16 = frozenset(_DTYPES)
+
+# These calls are a few microseconds of GPU work when the batch is small, so their host path is written for few Python
+# operations: each tensor is looked at once, in line.
+
+
+def _bad_cache(k, v, ks, vs, pages, b, dtype, index):
+    """The error of a cache or table that does not fit."""
+    if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _CACHE_DTYPES:
+        raise ValueError("Expected cache pools [n_pages, Hkv, page_size, D] of one type (BF16, FP16 or float8_e4m3fn)")
+    n, h, page, d = k.shape
+    if d not in (128, 256) or n < 1 or h < 1 or page < 16 or page % 16:
+        raise ValueError("Expected D=128/256 and a page size that is a multiple of 16")
+    if k.dtype is not _E8 and k.dtype != dtype:
+        raise ValueError("Expected a cache of the tensors' type, or of float8_e4m3fn")
+    if pages.ndim != 2 or pages.shape[0] != b or pages.shape[1] < 1 or pages.dtype != _INT or (
+            pages.shape[1] > 1 and pages.stride(1) != 1):
+        raise ValueError("Expected an int32 page table [B, max_pages] with contiguous rows")
+    if k.dtype is not _E8 and not (ks is None and vs is None):
+        raise ValueError("Scales belong to an e4m3 cache only")
+    if k.dtype is _E8 and (ks is None or vs is None or ks.shape != k.shape[:3] or vs.shape != k.shape[:3] or
+                           ks.dtype != _SCALE or vs.dtype != _SCALE):
+        raise ValueError("Expected float8_e8m0fnu scales [n_pages, Hkv, page_size] with an e4m3 cache")
+    raise ValueError("The cache and its table must lie on the tensors' CUDA device, with contiguous rows")
+
+
 def _cache_fields(cache, pages, b, dtype, index):
     """The kf_paged_cache of a call, after the checks that need no device."""
     if len(cache) == 2:
         (k, v), ks, vs = cache, None, None
     else:
         k, v, ks, vs = cache
-    if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _CACHE_DTYPES:
-        raise ValueError("Expected cache pools [n_pages, Hkv, page_size, D] of one type (BF16, FP16 or float8_e4m3fn)")
-    n, h, page, d = k.shape
-    if d not in (128, 256) or n < 1 or h < 1 or page < 16 or page % 16:
-        raise ValueError("Expected D=128/256 and a page size that is a multiple of 16")
-    e8 = k.dtype == torch.float8_e4m3fn
-    if not e8 and k.dtype != dtype:
-        raise ValueError("Expected a cache of the tensors' type, or of float8_e4m3fn")
-    if pages.ndim != 2 or pages.shape[0] != b or pages.shape[1] < 1 or pages.dtype != torch.int32 or (
-            pages.shape[1] > 1 and pages.stride(1) != 1):
-        raise ValueError("Expected an int32 page table [B, max_pages] with contiguous rows")
-    ok = k.is_cuda and k.get_device() == index and v.get_device() == index and pages.get_device() == index
-    sk, sv = k.stride(), v.stride()
-    ok = ok and sk[3] == 1 and sv[3] == 1
-    scale = (0, 0, 0, 0)
-    if e8:
-        if ks is None or vs is None or ks.shape != k.shape[:3] or vs.shape != k.shape[:3] or (
-                ks.dtype != torch.float8_e8m0fnu or vs.dtype != torch.float8_e8m0fnu):
-            raise ValueError("Expected float8_e8m0fnu scales [n_pages, Hkv, page_size] with an e4m3 cache")
-        ok = ok and ks.get_device() == index and vs.get_device() == index and ks.stride(2) == 1 and vs.stride(2) == 1
-        scale = ks.stride()[:2] + vs.stride()[:2]
-    elif ks is not None or vs is not None:
-        raise ValueError("Scales belong to an e4m3 cache only")
-    if not ok:
-        raise ValueError("The cache and its table must lie on the tensors' CUDA device, with contiguous rows")
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr() if e8 else 0, vs.data_ptr() if e8 else 0, pages.data_ptr(),
-            pages.stride(0), n, pages.shape[1], page, h, d, _CACHE_DTYPES[k.dtype], *sk[:3], *sv[:3], *scale)
+    shape, kind, sk, sv, sp, table = k.shape, k.dtype, k.stride(), v.stride(), pages.stride(), pages.shape
+    e8 = kind is _E8
+    ok = (len(shape) == 4 and v.shape == shape and v.dtype is kind and (e8 or kind is dtype) and len(table) == 2 and
+          table[0] == b and table[1] >= 1 and pages.dtype is _INT and (sp[1] == 1 or table[1] == 1) and
+          k.get_device() == v.get_device() == pages.get_device() == index >= 0 and sk[3] == 1 == sv[3])
+    if ok:
+        n, h, page, d = shape
+        ok = (d == 128 or d == 256) and n >= 1 and h >= 1 and page >= 16 and page % 16 == 0
+    if ok and e8:
+        ok = (ks is not None and vs is not None and ks.dtype is _SCALE and vs.dtype is _SCALE and
+              ks.shape == vs.shape == shape[:3] and ks.get_device() == vs.get_device() == index)
+        if ok:
+            a, c = ks.stride(), vs.stride()
+            if a[2] == 1 == c[2]:
+                return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages.data_ptr(), sp[0], n, table[1], page,
+                        h, d, _lib.KF_E4M3, sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], a[0], a[1], c[0], c[1])
+    elif ok and ks is None and vs is None:
+        return (k.data_ptr(), v.data_ptr(), 0, 0, pages.data_ptr(), sp[0], n, table[1], page, h, d, _DTYPES[kind], sk[0], sk[1],
+                sk[2], sv[0], sv[1], sv[2], 0, 0, 0, 0)
+    _bad_cache(k, v, ks, vs, pages, b, dtype, index)
 
 
 def _check_ints(name, t, b, index):
-    if t.dtype != torch.int32 or t.shape != (b,) or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not _INT or t.shape != (b,) or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"Expected {name} as contiguous int32 [B] on the tensors' CUDA device")
 
 
-def _check_rows(tensors):
-    """Every tensor in rows of a contiguous head dimension, on one CUDA device that is a B200, in one 16-bit type."""
-    first = tensors[0]
+def _check_rows(tensors, first, small):
+    """Every tensor in rows of a contiguous head dimension, on one CUDA device that is a B200, in one 16-bit type; the rows
+    that are read, weights and tables need no gradient."""
     dtype, index = first.dtype, first.get_device()
-    ok = dtype in _DTYPES and first.is_cuda
+    ok = dtype in _16 and index >= 0
     for t in tensors:
         if t.requires_grad:
             raise ValueError("This API is forward-only")
-        ok = ok and t.get_device() == index and t.dtype == dtype and t.stride(-1) == 1
+        ok = ok and t.get_device() == index and t.dtype is dtype and t.stride(-1) == 1
+    for t in small:
+        if t is not None:
+            if t.requires_grad:
+                raise ValueError("This API is forward-only")
+            ok = ok and t.get_device() == index and t.dtype is dtype and t.is_contiguous()
     if not ok:
         raise ValueError("Inputs must be BF16 (or FP16) with a contiguous head dimension on one CUDA device")
     if _major(index) != 10:
@@ -111,24 +136,25 @@ def _check_rows(tensors):
     return index
 
 
-def _small(d, gammas, cos, sin):
-    """Checks of weights and tables; the number of positions and the ones that are there."""
-    if (cos is None) != (sin is None):
-        raise ValueError("Provide both rotary tables or neither")
-    there = [g for g in gammas if g is not None]
-    for g in there:
-        if g.shape != (d,):
-            raise ValueError("Expected gamma [D]")
+def _check_small(d, gq, gk, cos, sin):
+    """Shapes of weights and tables; the number of positions."""
+    if (gq is not None and gq.shape != (d,)) or (gk is not None and gk.shape != (d,)):
+        raise ValueError("Expected gamma [D]")
     if cos is None:
-        return 0, there
-    if cos.ndim != 2 or cos.shape[1] != d or cos.shape[0] < 1 or sin.shape != cos.shape or not (
-            cos.is_contiguous() and sin.is_contiguous()):
+        if sin is not None:
+            raise ValueError("Provide both rotary tables or neither")
+        return 0
+    if sin is None:
+        raise ValueError("Provide both rotary tables or neither")
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != d or shape[0] < 1 or sin.shape != shape:
         raise ValueError("Expected contiguous rotary tables [positions, D]")
-    return cos.shape[0], [*there, cos, sin]
+    return shape[0]
 
 
-def _p(t):
-    return 0 if t is None else t.data_ptr()
+def _status_ptr(index):
+    w = _status.get(index)
+    return (status_word(torch.device("cuda", index)) if w is None else w).data_ptr()
 
 
 def append_rows(cache, k, v, pages, start, gk=None, cos=None, sin=None, *, counts=None, eps=1e-6):
@@ -141,21 +167,21 @@ def append_rows(cache, k, v, pages, start, gk=None, cos=None, sin=None, *, count
     if k.ndim != 4 or k.shape != v.shape or min(k.shape) < 1:
         raise ValueError("Expected K/V [B,Hkv,S,D]")
     b, h, s, d = k.shape
-    n_pos, small = _small(d, (gk,), cos, sin)
+    n_pos = _check_small(d, gk, None, cos, sin)
     if not (eps > 0):
         raise ValueError("eps must be positive")
-    index = _check_rows([k, v, *small])
+    index = _check_rows((k, v), k, (gk, cos, sin))
     fields = _cache_fields(cache, pages, b, k.dtype, index)
-    if cache[0].shape[1] != h or cache[0].shape[3] != d:
+    if fields[9] != h or fields[10] != d:
         raise ValueError("Expected K/V with the heads and the head dimension of the cache")
     _check_ints("start", start, b, index)
     if counts is not None:
         _check_ints("counts", counts, b, index)
+    packed = (k.data_ptr(), v.data_ptr(), 0 if gk is None else gk.data_ptr(), 0 if cos is None else cos.data_ptr(),
+              0 if sin is None else sin.data_ptr(), start.data_ptr(), 0 if counts is None else counts.data_ptr(),
+              _status_ptr(index), b, s, _DTYPES[k.dtype], n_pos)
     with _on_device(index):
-        _call(_lib.load().kf_append_rows(_APPEND.pack(
-            *fields, k.data_ptr(), v.data_ptr(), _p(gk), _p(cos), _p(sin), start.data_ptr(), _p(counts),
-            status_word(k.device).data_ptr(), b, s, _DTYPES[k.dtype], n_pos, *k.stride()[:3], *v.stride()[:3], eps),
-            _raw_stream(index)))
+        _call(_lib.load().kf_append_rows(_APPEND.pack(*fields, *packed, *k.stride()[:3], *v.stride()[:3], eps), _raw_stream(index)))
     return cache
 
 
@@ -181,12 +207,11 @@ def read_rows(cache, pages, lengths, s, *, dtype=None, k_out=None, v_out=None):
     v = torch.empty(shape, dtype=dtype, device=pool.device) if v_out is None else v_out
     if k.shape != shape or v.shape != shape or k.dtype != dtype or v.dtype != dtype:
         raise ValueError("k_out / v_out must be [B,Hkv,s,D] of the result's type")
-    _check_rows([k, v])
-    if k.get_device() != index:
+    if _check_rows((k, v), k, ()) != index:
         raise ValueError("k_out / v_out must lie on the cache's device")
     with _on_device(index):
         _call(_lib.load().kf_read_rows(_READ.pack(
-            *fields, k.data_ptr(), v.data_ptr(), lengths.data_ptr(), status_word(pool.device).data_ptr(), b, shape[2],
+            *fields, k.data_ptr(), v.data_ptr(), lengths.data_ptr(), _status_ptr(index), b, shape[2],
             _DTYPES[dtype], *k.stride()[:3], *v.stride()[:3]), _raw_stream(index)))
     return k, v
 
@@ -195,47 +220,56 @@ _workspace_bytes = {}  # (device, D, e4m3, more than eight query heads per KV he
 
 
 def _decode(q, new_k, new_v, cache, pages, lengths, gq, gk, cos, sin, eps, scale, out, workspace):
-    pool = cache[0]
-    if q.ndim != 4 or q.shape[2] != 1 or min(q.shape) < 1:
+    shape = q.shape
+    if len(shape) != 4 or shape[2] != 1 or shape[0] < 1 or shape[1] < 1:
         raise ValueError("Expected Q [B,Hq,1,D]: one token per sequence")
-    b, hq, _, d = q.shape
-    if pool.ndim != 4 or pool.shape[3] != d or pool.shape[1] < 1 or hq % pool.shape[1]:
+    b, hq, _, d = shape
+    pool = cache[0].shape
+    if len(pool) != 4 or pool[3] != d or pool[1] < 1 or hq % pool[1]:
         raise ValueError("Expected a cache of the queries' head dimension and valid GQA")
-    hkv = pool.shape[1]
-    n_pos, rows = _small(d, (gq, gk), cos, sin)
+    hkv = pool[1]
+    n_pos = _check_small(d, gq, gk, cos, sin)
     if not (eps > 0):
         raise ValueError("eps must be positive")
-    scale = d ** -0.5 if scale is None else scale
-    rows.insert(0, q)
-    strides = (0, 0, 0, 0)
-    if new_k is not None:
+    fresh = out is None
+    if fresh:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape:
+        raise ValueError("out must match q in shape and dtype")
+    if new_k is None:
+        index = _check_rows((q,) if fresh else (q, out), q, (gq, cos, sin))
+        new = (0, 0, 0)
+        new_strides = (0, 0, 0, 0)
+    else:
         if new_k.shape != (b, hkv, 1, d) or new_v.shape != new_k.shape:
             raise ValueError("Expected K/V [B,Hkv,1,D]: one token per sequence")
-        rows += (new_k, new_v)
-        strides = new_k.stride()[:2] + new_v.stride()[:2]
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape:
-        raise ValueError("out must match q in shape and dtype")
-    rows.append(out)
-    index = _check_rows(rows)
+        index = _check_rows((q, new_k, new_v) if fresh else (q, new_k, new_v, out), q, (gq, gk, cos, sin))
+        new = (new_k.data_ptr(), new_v.data_ptr(), 0 if gk is None else gk.data_ptr())
+        nk, nv = new_k.stride(), new_v.stride()
+        new_strides = (nk[0], nk[1], nv[0], nv[1])
     fields = _cache_fields(cache, pages, b, q.dtype, index)
     _check_ints("lengths", lengths, b, index)
     lib = _lib.load()
-    with _on_device(index):
-        key = (index, d, fields[11], hq > 8 * hkv)
-        need = _workspace_bytes.get(key)
-        if need is None:
-            need = _workspace_bytes[key] = lib.kf_decode_workspace_bytes(b, hq, hkv, d, fields[11])
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        elif (workspace.numel() * workspace.element_size() < need or workspace.get_device() != index or
-              not workspace.is_contiguous()):
-            raise ValueError(f"workspace must be contiguous, on the queries' device and hold {need} bytes")
-        _call(lib.kf_decode_attention(_DECODE.pack(
-            *fields, q.data_ptr(), _p(gq), _p(cos), _p(sin), out.data_ptr(), lengths.data_ptr(), _p(new_k), _p(new_v),
-            _p(gk), workspace.data_ptr(), status_word(q.device).data_ptr(), b, hq, _DTYPES[q.dtype], n_pos,
-            *q.stride()[:2], *out.stride()[:2], *strides, eps, scale), _raw_stream(index)))
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _decode(q, new_k, new_v, cache, pages, lengths, gq, gk, cos, sin, eps, scale, out, workspace)
+    key = (index, d, fields[11], hq > 8 * hkv)
+    need = _workspace_bytes.get(key)
+    if need is None:
+        need = _workspace_bytes[key] = lib.kf_decode_workspace_bytes(b, hq, hkv, d, fields[11])
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif (workspace.numel() * workspace.element_size() < need or workspace.get_device() != index or
+          not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be contiguous, on the queries' device and hold {need} bytes")
+    sq, so = q.stride(), out.stride()
+    rc = lib.kf_decode_attention(_DECODE.pack(
+        *fields, q.data_ptr(), 0 if gq is None else gq.data_ptr(), 0 if cos is None else cos.data_ptr(),
+        0 if sin is None else sin.data_ptr(), out.data_ptr(), lengths.data_ptr(), *new, workspace.data_ptr(),
+        _status_ptr(index), b, hq, _DTYPES[q.dtype], n_pos, sq[0], sq[1], so[0], so[1], *new_strides, eps,
+        d ** -0.5 if scale is None else scale), _raw_stream(index))
+    if rc:
+        _call(rc)
     return out
 
 
