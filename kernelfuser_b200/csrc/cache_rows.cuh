@@ -9,6 +9,8 @@
 // up to a factor of two earlier) and makes scaling exact, so that each value is rounded once and reading back to 16
 // bits is exact.  (Magnitudes above 448 * 2^119 = 2.98e38 become that.)  A row whose largest magnitude is not finite gets the NaN scale and reads back as NaN.
 #pragma once
+#include <type_traits>
+
 #include "ptx.cuh"
 #include "rounding.cuh"
 
@@ -133,14 +135,15 @@ template <int D, int LPR> struct Row {
     }
     // bits of the largest magnitude of the row (a NaN is the largest)
     __device__ __forceinline__ uint32_t largest() const {
-        uint32_t m = 0;
+        float m = 0.f;
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int i = 0; i < W; ++i) m = max(m, __float_as_uint(x[half][i]) & 0x7fffffffu);
+            for (int i = 0; i < W; ++i) asm("max.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(m) : "f"(x[half][i]));
+        uint32_t bits = __float_as_uint(m) & 0x7fffffffu;
 #pragma unroll
-        for (int d = 1; d < LPR; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        return m;
+        for (int d = 1; d < LPR; d *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+        return bits;
     }
     // The row in the cache's type: `put(byte offset, value)` with a value of 2, 4, 8 or 16 bytes.  Returns the scale's byte.
     template <typename T, bool E8, typename F> __device__ __forceinline__ uint32_t store(int lane, F&& put) const {
@@ -186,31 +189,47 @@ struct AppendArgs {
 
 constexpr int kRowsThreads = 256;
 
-// A group of D/16 lanes walks over heads of one position, so that the tables are read once for them; a lane's columns are
-// two 16-byte pieces of a row.
+// A group of D/16 lanes takes up to kAppendHeads heads of one position, so that the tables are read once for them and their rows
+// are in flight together; K rows and V rows are different CTAs' work (blockIdx.z).
+constexpr int kAppendHeads = 4;
+
 template <int D, typename T, bool E8>
 __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendArgs a) {
     constexpr int LPR = D / 16;
-    if (*reinterpret_cast<volatile int*>(a.status) != 0) return;
+    using R = Row<D, LPR>;
+    const int failed = *reinterpret_cast<volatile int*>(a.status);  // (looked at when there is something to write)
+    const bool is_k = blockIdx.z == 0;
     const int sub = threadIdx.x % LPR;
     const long long task = static_cast<long long>(blockIdx.x) * (kRowsThreads / LPR) + threadIdx.x / LPR;
     const int b = static_cast<int>(task / a.S), s = static_cast<int>(task - static_cast<long long>(b) * a.S);
     bool valid = b < a.B;
+    int start = 0, count = 0;
+    if (valid) {
+        start = __ldg(a.start + b);
+        count = a.counts != nullptr ? __ldg(a.counts + b) : a.S;
+    }
+    valid = s < count;
+    // the rows are asked for before their place is known
+    const int h0 = blockIdx.y * a.heads_per_group, heads = min(a.heads_per_group, a.H - h0);
+    const T* const src = is_k ? reinterpret_cast<const T*>(a.k) + b * a.k_sb + s * a.k_ss + h0 * a.k_sh
+                              : reinterpret_cast<const T*>(a.v) + b * a.v_sb + s * a.v_ss + h0 * a.v_sh;
+    const long long src_h = is_k ? a.k_sh : a.v_sh;
+    typename R::Words rows[kAppendHeads] = {};
+#pragma unroll
+    for (int i = 0; i < kAppendHeads; ++i)
+        if (valid && i < heads) R::template load<true>(rows[i], src + i * src_h, sub);
     int pos = 0, page = 0, row = 0;
     if (valid) {
-        if (a.counts != nullptr) valid = s < a.counts[b];
-        const long long p = static_cast<long long>(a.start[b]) + s;
-        if (valid && (p < 0 || p >= a.c.capacity)) {
+        const long long p = static_cast<long long>(start) + s;
+        if (p < 0 || p >= a.c.capacity) {
             report(a.status, kStatusBadLength);
             valid = false;
-        }
-        pos = static_cast<int>(p);
-        if (valid && a.cos != nullptr && pos >= a.n_pos) {
+        } else if (a.cos != nullptr && p >= a.n_pos) {
             report(a.status, kStatusBadPosition);
             valid = false;
-        }
-        if (valid) {
-            page = a.c.pages[b * a.c.pages_sb + pos / a.c.page_size];
+        } else {
+            pos = static_cast<int>(p);
+            page = __ldg(a.c.pages + b * a.c.pages_sb + pos / a.c.page_size);
             row = pos % a.c.page_size;
             if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
                 report(a.status, kStatusBadPage);
@@ -218,40 +237,32 @@ __global__ void __launch_bounds__(kRowsThreads) append_rows_kernel(const AppendA
             }
         }
     }
-    using R = Row<D, LPR>;
     typename R::Words gamma, cos, sin;
-    if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, sub);
-    if (a.cos != nullptr) {
-        R::template load<false>(cos, reinterpret_cast<const T*>(a.cos) + static_cast<long long>(valid ? pos : 0) * D, sub);
-        R::template load<false>(sin, reinterpret_cast<const T*>(a.sin) + static_cast<long long>(valid ? pos : 0) * D, sub);
+    if (is_k && a.gamma != nullptr) R::template load<false>(gamma, a.gamma, sub);
+    if (is_k && a.cos != nullptr) {
+        R::template load<false>(cos, reinterpret_cast<const T*>(a.cos) + static_cast<long long>(pos) * D, sub);
+        R::template load<false>(sin, reinterpret_cast<const T*>(a.sin) + static_cast<long long>(pos) * D, sub);
     }
-    const int h0 = blockIdx.y * a.heads_per_group, h1 = min(h0 + a.heads_per_group, a.H);
-    const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_sb + s * a.k_ss;
-    const T* vb = reinterpret_cast<const T*>(a.v) + b * a.v_sb + s * a.v_ss;
-    unsigned char* kd = a.c.k + wide(page, a.c.k_sp) + wide(row, a.c.k_ss);
-    unsigned char* vd = a.c.v + wide(page, a.c.v_sp) + wide(row, a.c.v_ss);
-    for (int h = h0; h < h1; ++h) {
-        typename R::Words kw = {}, vw = {};
-        if (valid) {
-            R::template load<true>(kw, kb + h * a.k_sh, sub);
-            R::template load<true>(vw, vb + h * a.v_sh, sub);
-        }
-        R k, v;
-        k.template unpack<T>(kw);
-        v.template unpack<T>(vw);
-        if (a.gamma != nullptr) k.template norm<T>(gamma, a.eps);
-        if (a.cos != nullptr) k.template rotate<T>(cos, sin);
-        auto to = [&](unsigned char* dst) {
-            return [=](int at, auto value) {
-                if (valid) *reinterpret_cast<decltype(value)*>(dst + at) = value;
-            };
-        };
-        const uint32_t ke = k.template store<T, E8>(sub, to(kd + wide(h, a.c.k_sh)));
-        const uint32_t ve = v.template store<T, E8>(sub, to(vd + wide(h, a.c.v_sh)));
-        if (E8 && valid && sub == 0) {
-            a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row] = static_cast<unsigned char>(ke);
-            a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row] = static_cast<unsigned char>(ve);
-        }
+    valid = valid && failed == 0;
+    unsigned char* dst = is_k ? a.c.k + wide(page, a.c.k_sp) + wide(row, a.c.k_ss) + wide(h0, a.c.k_sh)
+                              : a.c.v + wide(page, a.c.v_sp) + wide(row, a.c.v_ss) + wide(h0, a.c.v_sh);
+    unsigned char* scale = nullptr;
+    if constexpr (E8)
+        scale = is_k ? a.c.k_scale + wide(page, a.c.ks_sp) + wide(h0, a.c.ks_sh) + row : a.c.v_scale + wide(page, a.c.vs_sp) + wide(h0, a.c.vs_sh) + row;
+    const int dst_h = is_k ? a.c.k_sh : a.c.v_sh, scale_h = is_k ? a.c.ks_sh : a.c.vs_sh;
+#pragma unroll
+    for (int i = 0; i < kAppendHeads; ++i) {
+        if (i >= heads) break;
+        R x;
+        x.template unpack<T>(rows[i]);
+        if (is_k && a.gamma != nullptr) x.template norm<T>(gamma, a.eps);
+        if (is_k && a.cos != nullptr) x.template rotate<T>(cos, sin);
+        const uint32_t e = x.template store<T, E8>(sub, [&](int at, auto value) {
+            if (valid) *reinterpret_cast<decltype(value)*>(dst + at) = value;
+        });
+        if (E8 && valid && sub == 0) *scale = static_cast<unsigned char>(e);
+        dst += dst_h;
+        if constexpr (E8) scale += scale_h;
     }
 }
 
@@ -264,15 +275,17 @@ struct ReadArgs {
     int* status;
 };
 
-constexpr int kReadUnroll = 4;  // rows of K and of V in flight per lane
+// A lane owns 8 columns of a row: one 16-byte store, and a 16-byte (16-bit cache) or 8-byte load.  A CTA takes some blocks of
+// rows of one head of one sequence; a block lies in one page, whose place is looked up once for all its lanes.
+constexpr int kReadBlocks = 4;  // in flight per lane, of K and of V
+template <int D> __host__ __device__ constexpr int read_block() { return kRowsThreads / (D / 8); }  // rows; divides 16
 
-// A lane owns 8 columns of a row: one 16-byte store, and a 16-byte (16-bit cache) or 8-byte load.  A CTA takes
-// kReadUnroll * (threads / lanes per row) rows of one head of one sequence.
 template <int D, typename T, bool E8>
 __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs a) {
-    constexpr int LPR = D / 8, RPB = kRowsThreads / LPR;
-    if (*reinterpret_cast<volatile int*>(a.status) != 0) return;
-    const int sub = threadIdx.x % LPR, r0 = blockIdx.x * (RPB * kReadUnroll) + threadIdx.x / LPR;
+    constexpr int LPR = D / 8, RPB = read_block<D>();
+    using Raw = typename std::conditional<E8, uint2, uint4>::type;
+    const int failed = *reinterpret_cast<volatile int*>(a.status);  // (looked at when there is something to write)
+    const int sub = threadIdx.x % LPR, r = threadIdx.x / LPR, first = blockIdx.x * (RPB * kReadBlocks);
     for (long long bh = blockIdx.y; bh < static_cast<long long>(a.B) * a.H; bh += gridDim.y) {
         const int b = static_cast<int>(bh / a.H), h = static_cast<int>(bh - static_cast<long long>(b) * a.H);
         int len = a.lengths[b];
@@ -280,58 +293,51 @@ __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs 
             report(a.status, kStatusBadLength);
             len = a.c.capacity;
         }
-        uint4 kx[kReadUnroll], vx[kReadUnroll];
-        float kf[kReadUnroll], vf[kReadUnroll];
+        len = min(len, a.S);
+        const unsigned char* const kh = a.c.k + wide(h, a.c.k_sh) + wide(r, a.c.k_ss);
+        const unsigned char* const vh = a.c.v + wide(h, a.c.v_sh) + wide(r, a.c.v_ss);
+        Raw kx[kReadBlocks], vx[kReadBlocks];
+        float kf[kReadBlocks], vf[kReadBlocks];
 #pragma unroll
-        for (int u = 0; u < kReadUnroll; ++u) {
-            const int s = r0 + u * RPB;
-            kx[u] = vx[u] = make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < kReadBlocks; ++u) {
+            const int s0 = first + u * RPB;
+            kx[u] = vx[u] = Raw{};
             kf[u] = vf[u] = 0.f;
-            if (s >= a.S || s >= len) continue;
-            const int page = a.c.pages[b * a.c.pages_sb + s / a.c.page_size], row = s % a.c.page_size;
+            if (s0 >= len) continue;  // (all lanes alike)
+            const int i = s0 / a.c.page_size, row = s0 - i * a.c.page_size, page = __ldg(a.c.pages + b * a.c.pages_sb + i);
             if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
                 report(a.status, kStatusBadPage);
                 continue;
             }
-            const unsigned char* kp = a.c.k + wide(page, a.c.k_sp) + wide(h, a.c.k_sh) + wide(row, a.c.k_ss);
-            const unsigned char* vp = a.c.v + wide(page, a.c.v_sp) + wide(h, a.c.v_sh) + wide(row, a.c.v_ss);
+            if (s0 + r >= len) continue;
+            kx[u] = __ldcs(reinterpret_cast<const Raw*>(kh + wide(page, a.c.k_sp) + wide(row, a.c.k_ss)) + sub);
+            vx[u] = __ldcs(reinterpret_cast<const Raw*>(vh + wide(page, a.c.v_sp) + wide(row, a.c.v_ss)) + sub);
             if constexpr (E8) {
-                const uint2 k2 = __ldcs(reinterpret_cast<const uint2*>(kp) + sub);
-                const uint2 v2 = __ldcs(reinterpret_cast<const uint2*>(vp) + sub);
-                kx[u].x = k2.x;
-                kx[u].y = k2.y;
-                vx[u].x = v2.x;
-                vx[u].y = v2.y;
-                kf[u] = scale_value(a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row]);
-                vf[u] = scale_value(a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row]);
-            } else {
-                kx[u] = __ldcs(reinterpret_cast<const uint4*>(kp) + sub);
-                vx[u] = __ldcs(reinterpret_cast<const uint4*>(vp) + sub);
+                kf[u] = scale_value(a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row + r]);
+                vf[u] = scale_value(a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row + r]);
             }
         }
-        auto widen = [](uint4& x, float f) {
-            const uint32_t w[4] = {x.x, x.x >> 16, x.y, x.y >> 16};
-            uint32_t o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t h2 = e4m3_to_half2(w[i]);
-                const float2 y = Num<__half>::unpack(h2);
-                o[i] = Num<T>::pack(y.x * f, y.y * f);
-            }
-            x = make_uint4(o[0], o[1], o[2], o[3]);
-        };
-#pragma unroll
-        for (int u = 0; u < kReadUnroll; ++u) {
-            const int s = r0 + u * RPB;
-            if (s >= a.S) continue;
+        auto put = [&](T* row, const Raw& x, float f) {
             if constexpr (E8) {
-                widen(kx[u], kf[u]);
-                widen(vx[u], vf[u]);
+                const uint32_t w[4] = {x.x, x.x >> 16, x.y, x.y >> 16};
+                uint32_t o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 y = Num<__half>::unpack(e4m3_to_half2(w[i]));
+                    o[i] = Num<T>::pack(y.x * f, y.y * f);
+                }
+                __stcs(reinterpret_cast<uint4*>(row) + sub, make_uint4(o[0], o[1], o[2], o[3]));
+            } else {
+                __stcs(reinterpret_cast<uint4*>(row) + sub, x);
             }
-            T* ko = reinterpret_cast<T*>(a.k) + b * a.k_sb + h * a.k_sh + s * a.k_ss;
-            T* vo = reinterpret_cast<T*>(a.v) + b * a.v_sb + h * a.v_sh + s * a.v_ss;
-            __stcs(reinterpret_cast<uint4*>(ko) + sub, kx[u]);
-            __stcs(reinterpret_cast<uint4*>(vo) + sub, vx[u]);
+        };
+        T* const ko = reinterpret_cast<T*>(a.k) + b * a.k_sb + h * a.k_sh + (first + r) * a.k_ss;
+        T* const vo = reinterpret_cast<T*>(a.v) + b * a.v_sb + h * a.v_sh + (first + r) * a.v_ss;
+#pragma unroll
+        for (int u = 0; u < kReadBlocks; ++u) {
+            if (first + r + u * RPB >= a.S || failed != 0) continue;
+            put(ko + u * RPB * a.k_ss, kx[u], kf[u]);
+            put(vo + u * RPB * a.v_ss, vx[u], vf[u]);
         }
     }
 }

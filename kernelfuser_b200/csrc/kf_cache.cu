@@ -97,15 +97,16 @@ template <int D, typename T, bool E8> int launch_append(const kf::AppendArgs& a,
     constexpr int kTasks = kf::kRowsThreads / (D / 16);
     const long long gx = (static_cast<long long>(a.B) * a.S + kTasks - 1) / kTasks;
     kf::AppendArgs args = a;
-    // One head per group while that is what fills the SMs; all heads of a position (one reading of the tables) once there
-    // are eight CTAs an SM without splitting them.
-    args.heads_per_group = gx >= 8LL * sm_count() ? a.H : 1;
+    // One head to a group of lanes while that is what spreads the rows over the SMs, several (the tables are then read once
+    // for them, and as many rows are in flight) once there are two CTAs an SM that way.
+    args.heads_per_group = gx * ((a.H + kf::kAppendHeads - 1) / kf::kAppendHeads) >= sm_count() ? kf::kAppendHeads : 1;
     const unsigned gy = (unsigned)((a.H + args.heads_per_group - 1) / args.heads_per_group);
-    return launched("append_rows", launch_kernel(kf::append_rows_kernel<D, T, E8>, dim3((unsigned)gx, gy), dim3(kf::kRowsThreads), 0, st, args));
+    if (gy > 65535) return fail(KF_EINVAL, "too many heads");
+    return launched("append_rows", launch_kernel(kf::append_rows_kernel<D, T, E8>, dim3((unsigned)gx, gy, 2), dim3(kf::kRowsThreads), 0, st, args));
 }
 
 template <int D, typename T, bool E8> int launch_read(const kf::ReadArgs& a, cudaStream_t st) {
-    constexpr int kRows = kf::kRowsThreads / (D / 8) * kf::kReadUnroll;
+    constexpr int kRows = kf::read_block<D>() * kf::kReadBlocks;
     const unsigned gx = (unsigned)((a.S + kRows - 1) / kRows);
     const long long bh = static_cast<long long>(a.B) * a.H;
     return launched("read_rows", launch_kernel(kf::read_rows_kernel<D, T, E8>, dim3(gx, (unsigned)(bh < 65535 ? bh : 65535)),
