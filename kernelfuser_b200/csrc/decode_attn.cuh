@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     {
         const int per_lane = (a.B + 31) / 32, b_lo = lane * per_lane;
         unsigned int mine = 0, rows_at_all = 0;
+#pragma unroll 8
         for (int b = b_lo; b < min(b_lo + per_lane, a.B); ++b) {
             const int n = __ldg(a.lengths + b);
             if (n > a.c.capacity) report(a.status, kStatusBadLength);
