@@ -163,6 +163,9 @@ template <int UNIT, int COST> struct DecodeCursor {
     }
 };
 
+// An f16 product of a bf16 call needs no second part: its own rounding is an eighth of what the output's costs.
+template <typename T, bool E8> constexpr bool kSplitProducts = !(E8 && std::is_same<T, __nv_bfloat16>::value);
+
 // Two values, each as high + low of the products' type: high is rounded towards zero, so that low has the value's sign and
 // together they hold twice the type's bits.  A low part that would be zero becomes the type's smallest number instead
 // (kMin, far below what is kept): an infinity in the cache then meets two factors of one sign and stays that infinity.
@@ -255,7 +258,9 @@ template <int D, typename T, int NT> struct QueryRows {
                     const int col = half * (D / 2) + lane * R::W + 2 * p, in = col % 16;
                     const int t = E8 ? in / 4 : in % 8 / 2, reg = E8 ? in % 4 / 2 : in / 8;
                     uint32_t* const dst = reinterpret_cast<uint32_t*>(frag + (r / 8 * (D / 16) + col / 16) * 32 + r % 8 * 4 + t);
-                    split2<M>(row.x[half][2 * p] * up, row.x[half][2 * p + 1] * up, dst[reg], dst[reg + 2]);
+                    const float x0 = row.x[half][2 * p] * up, x1 = row.x[half][2 * p + 1] * up;
+                    if constexpr (kSplitProducts<T, E8>) split2<M>(x0, x1, dst[reg], dst[reg + 2]);
+                    else dst[reg] = Num<M>::pack(x0, x1);
                 }
         }
     }
@@ -698,8 +703,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     // Probabilities are 2^(score - base + kUp), the base at most kSlack behind the largest score so far: up to 2^15 in f16,
     // whose smallest step is then 2^-35 of the largest probability, up to 2^8 in bf16.
     constexpr bool kHalf = std::is_same<M, __half>::value;
-    // An f16 product of a bf16 call needs no second part: its own is an eighth of what rounding the output to bf16 loses.
-    constexpr bool kSplit = !(E8 && std::is_same<T, __nv_bfloat16>::value);
+    constexpr bool kSplit = kSplitProducts<T, E8>;
     constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : 0.f;
 
     while (cc.left > 0) {
