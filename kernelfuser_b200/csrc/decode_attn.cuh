@@ -732,12 +732,14 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         // m, mv: bases of the sum and of O (an 8-bit cache's value scales belong to the latter), -inf before the first key
         float o[NT][kDT][4], m[NT][2], mv[NT][2], l[NT][2];
         float off[NT][2], off_v[NT][2];  // kUp - base, what is added to a score
+        float lim[NT][2], lim_v[NT][2];  // base + kSlack: a score above it moves the base
 #pragma unroll
         for (int u = 0; u < NT; ++u) {
 #pragma unroll
             for (int i = 0; i < kDT; ++i) o[u][i][0] = o[u][i][1] = o[u][i][2] = o[u][i][3] = 0.f;
             m[u][0] = m[u][1] = mv[u][0] = mv[u][1] = -INFINITY;
             off[u][0] = off[u][1] = off_v[u][0] = off_v[u][1] = 0.f;
+            lim[u][0] = lim[u][1] = lim_v[u][0] = lim_v[u][1] = -INFINITY;
             l[u][0] = l[u][1] = 0.f;
         }
         // the new token's step is the last one with keys, in the item's last unit
@@ -765,6 +767,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                         if constexpr (kSplit) mma16816<M>(s[u][tile][1], a0, a1, a2, a3, f.z, f.w);
                     }
                 };
+                float scale = 1.f;  // of key `lane` of the step
+                if constexpr (E8) scale = scale_value(scales[slot * C::kKeys + lane]);
                 const uint32_t k_at = k_lane + slot * C::kSlotBytes;
 #pragma unroll
                 for (int j = 0; j < kDT; j += E8 ? 2 : 1)
@@ -788,8 +792,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                 for (int tile = 0; tile < C::kTiles; ++tile) {
                     float f0 = 1.f, f1 = 1.f;  // scales of the keys
                     if constexpr (E8) {
-                        f0 = scale_value(scales[slot * C::kKeys + 16 * tile + g]);
-                        f1 = scale_value(scales[slot * C::kKeys + 16 * tile + g + 8]);
+                        f0 = __shfl_sync(0xffffffffu, scale, 16 * tile + g);
+                        f1 = __shfl_sync(0xffffffffu, scale, 16 * tile + g + 8);
                     }
 #pragma unroll
                     for (int u = 0; u < NT; ++u)
@@ -813,18 +817,18 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             if (keys > 0) {
                 bool above = false;
                 if constexpr (E8) {
+                    // exponent of value row `lane` of the step (2^23 + e as bits: e - 127 without a conversion)
+                    const uint32_t e = scales[slot * C::kKeys + lane];
+                    const float exponent = e == 255 ? NAN : __uint_as_float(0x4b000000u | e) - 8388735.f;
 #pragma unroll
                     for (int tile = 0; tile < C::kTiles; ++tile) {
-                        const uint32_t e0 = scales[slot * C::kKeys + 16 * tile + g], e1 = scales[slot * C::kKeys + 16 * tile + g + 8];
-                        // (2^23 + e as bits: e - 127 without a conversion)
-                        const float ve0 = e0 == 255 ? NAN : __uint_as_float(0x4b000000u | e0) - 8388735.f;
-                        const float ve1 = e1 == 255 ? NAN : __uint_as_float(0x4b000000u | e1) - 8388735.f;
+                        const float ve0 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g), ve1 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g + 8);
 #pragma unroll
                         for (int u = 0; u < NT; ++u)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 w[u][tile][i] = x[u][tile][i] + (i < 2 ? ve0 : ve1);
-                                above |= w[u][tile][i] > mv[u][i & 1] + kSlack;
+                                above |= w[u][tile][i] > lim_v[u][i & 1];
                             }
                     }
                     if (keys < C::kKeys) {  // (scales behind the sequence are whatever the page holds)
@@ -838,7 +842,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
-                    for (int i = 0; i < 4 * C::kTiles; ++i) above |= x[u][i / 4][i % 4] > m[u][i & 1] + kSlack;
+                    for (int i = 0; i < 4 * C::kTiles; ++i) above |= x[u][i / 4][i % 4] > lim[u][i & 1];
                 if (__any_sync(0xffffffffu, above)) {  // move the bases (of the heads whose own scores ask for it) to the maxima
                     auto top = [](const float (&y)[C::kTiles][4], int c, float base) {
                         float z = fmaxf(y[0][c], y[0][c + 2]);
@@ -866,6 +870,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                             mv[u][c] = to_v;
                             off[u][c] = to == -INFINITY ? 0.f : kUp - to;
                             off_v[u][c] = to_v == -INFINITY ? 0.f : kUp - to_v;
+                            lim[u][c] = to + kSlack;
+                            lim_v[u][c] = to_v + kSlack;
                         }
                 }
                 uint32_t pb[NT][C::kTiles][4];  // high and low part of the probabilities of keys 0-7, 8-15
