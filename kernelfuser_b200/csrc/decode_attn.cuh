@@ -75,7 +75,7 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     // give the schedulers a third warp each (135 -> 116 us with steps of 16; four, at 128 registers: 124).
     // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
     static constexpr int kSlots = E8 ? (D == 128 ? (NT == 1 ? 3 : 5) : 3) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
-    static constexpr int kMergeCols = D == 256 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
+    static constexpr int kMergeCols = D == 256 || E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
     static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
@@ -292,7 +292,11 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
 
     // parts that the ring holds side by side, of rows that exist
     __device__ __forceinline__ int part_floats() const { return min(kRows, a.G) * D + 2 * kRows; }
-    __device__ __forceinline__ int join_group() const { return min(64, C::kRingBytes / 4 / part_floats()); }
+    // Parts that one CTA joins of an item of n: all, if its ring holds them, else about as many as there will be groups (32
+    // parts of 4 KB: 7 us one ring full after the other, 5 in six groups of six).
+    __device__ __forceinline__ int join_group(int n) const {
+        return n <= min(64, C::kRingBytes / 4 / part_floats()) ? n : static_cast<int>(ceilf(sqrtf(static_cast<float>(n))));
+    }
 
     // One thread: count one more in the field; true for the CTA that completes `count`.
     __device__ __forceinline__ bool count_up(int cta, int shift, int count) const {
@@ -372,14 +376,14 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     }
     // All threads, once: this CTA's parts are in their places (`dead`: they never will be; only the counts have to go on).
     __device__ __forceinline__ void parts_done(const DecodeBroken (&item)[2], bool dead) const {
-        const int cta = blockIdx.x, group = join_group();
+        const int cta = blockIdx.x;
         __syncthreads();
         if (threadIdx.x == 0 || threadIdx.x == 32) {  // (a lane of its own for each: the two round trips overlap)
             __threadfence();  // the CTA's parts are visible before they count
             const DecodeBroken& it = item[threadIdx.x / 32];
             bool all = false;
             if (it.first >= 0) {
-                const int from = it.first + (cta - it.first) / group * group, n = min(group, it.last - from + 1);
+                const int group = join_group(it.last - it.first + 1), from = it.first + (cta - it.first) / group * group, n = min(group, it.last - from + 1);
                 all = n == 1 || count_up(from, from == it.first ? 8 : 0, n);
             }
             __threadfence();
@@ -390,7 +394,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
         for (int k = 0; k < 2; ++k) {
             if (s_flag[k] == 0) continue;
             const DecodeBroken it = k == 0 ? item[0] : item[1];
-            const int groups = (it.last - it.first) / group + 1, row0 = (it.hk - it.h * a.row_blocks) * kRows;
+            const int group = join_group(it.last - it.first + 1), groups = (it.last - it.first) / group + 1, row0 = (it.hk - it.h * a.row_blocks) * kRows;
             int from = it.first + (cta - it.first) / group * group, stride = 1, n = min(group, it.last - from + 1);
             bool final = groups == 1;
 #pragma unroll 1
