@@ -13,8 +13,8 @@
 // order of the line whoever that is: as many at a time as its ring holds, and if there are more, the joined groups once more.  (A second kernel
 // for it cost 2 us of a call, and its serial pass over 37 parts of a long sequence 12 us.)
 //
-// Inside a CTA each of the four warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
-// into its own ring of slots in shared memory (cp.async, across item borders), and keeps its own sum and output; the four
+// Inside a CTA each of the four (or eight) warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
+// into its own ring of slots in shared memory (cp.async, across item borders), and keeps its own sum and output; they
 // meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are the m16 of mma.m16n8k16 and the
 // query heads its n8, so up to eight heads cost one instruction per 16 x 16 block of the cache.  (The 128-row MMAs of the
 // prefill kernels have nothing to fill their rows with here.)  Q is prepared once per item, a row to a warp, from values
@@ -53,14 +53,15 @@ struct DecodeArgs {
     int* status;
 };
 
-constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
 // Items of up to this many units are not broken for CTAs that would be idle: joining costs about as much as four units of one
 // warp each (3 units: 8.7 us whole, 9.7 broken).  Longer ones are, down to single units (128 units 17.8 -> 14.8 us, 16: 13.4 -> 11.4).
 constexpr int kDecWhole = 4;
 
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
-    static constexpr int kTiles = E8 ? 2 : 1, kKeys = 16 * kTiles, kUnit = kKeys * kDecWarps;  // keys of a warp's step, of a unit
+    static constexpr bool kWide = D == 256 && NT == 2;                // more than eight heads of 256
+    static constexpr int kWarps = kWide ? 8 : 4, kThreads = 32 * kWarps;
+    static constexpr int kTiles = E8 && !kWide ? 2 : 1, kKeys = 16 * kTiles, kUnit = kKeys * kWarps;  // keys of a warp's step, of a unit
     static constexpr int kRowBytes = D * (E8 ? 1 : 2);
     // What an item costs beside its units, in units of its keys: about 3 us of a CTA (looking up its rows, preparing its
     // queries, meeting of the warps), which hold a unit of 64 KB or two of 32.  32 ragged sequences of up to 1500 rows: 1 -> 36
@@ -68,18 +69,19 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kItemCost = kRowBytes == 512 ? 2 : 3;
     static constexpr int kSlotBytes = kKeys * kRowBytes;              // K or V rows of a step
     static constexpr int kScaleBytes = E8 ? kKeys : 0;                // and their scales
-    static constexpr bool kQueryInRegs = D * NT <= 256;               // else its fragments are read for every step
-    static constexpr int kCtasPerSm = E8 && D == 128 && NT == 1 ? 3 : kQueryInRegs ? 2 : 1;
+    static constexpr bool kQueryInRegs = !kWide;                      // else its fragments are read for every step
+    static constexpr int kCtasPerSm = kWide ? 1 : E8 && D == 128 && NT == 1 ? 3 : 2;
     // An 8-bit cache is bound by the instructions that widen it as much as by HBM: steps of 32 keys share what a step costs
     // and have twice as many independent products (64 sequences of 4096 rows, G = 4: 118 -> 98 us, floor 83), and three CTAs
     // give the schedulers a third warp each (135 -> 116 us with steps of 16; four, at 128 registers: 124).
+    // With more than eight heads of 256 O alone takes 128 registers and one CTA's queries 16 KB: eight warps share them.
     // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
-    static constexpr int kSlots = E8 ? (D == 128 ? (NT == 1 ? 3 : 5) : 3) : kQueryInRegs ? (D == 256 ? 3 : NT == 1 ? 6 : 5) : 6;
+    static constexpr int kSlots = E8 ? (kWide || (D == 128 && NT == 2) ? 5 : 3) : D == 256 ? 3 : NT == 1 ? 6 : 5;
     static constexpr int kMergeCols = D == 256 || E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
-    static constexpr int kRingBytes = kDecWarps * kSlots * kSlotBytes;
-    static constexpr int kScaleRingBytes = kDecWarps * kSlots * kScaleBytes;
+    static constexpr int kRingBytes = kWarps * kSlots * kSlotBytes;
+    static constexpr int kScaleRingBytes = kWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
-    static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kDecWarps + 1) * kRows * 4;
+    static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kWarps + 1) * kRows * 4;
     static constexpr int kNewBytes = 2 * kRowBytes;                   // a new token's K and V row
     static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes + kNewBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
@@ -209,16 +211,16 @@ template <typename M, bool FLOOR> __device__ __forceinline__ void split2_probabi
     low = FLOOR ? Num<M>::pack(fmaxf(x, Split<M>::kMin), fmaxf(y, Split<M>::kMin)) : Num<M>::pack(x, y);
 }
 
-// The query rows that a warp prepares for an item (row, row + 4, ...), loaded ahead of time.
-template <int D, typename T, int NT> struct QueryRows {
+// The query rows that a warp prepares for an item (every WARPS-th), loaded ahead of time.
+template <int D, typename T, int NT, int WARPS> struct QueryRows {
     using R = Row<D, 32>;
-    static constexpr int kN = 2 * NT;  // rows of a warp
+    static constexpr int kN = 8 * NT / WARPS;  // rows of a warp
     typename R::Words q[kN], cos, sin;
     template <typename Cursor> __device__ __forceinline__ void load(const DecodeArgs& a, const Cursor& at) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = (at.hk - at.h * a.row_blocks) * 8 * NT;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int r = row0 + warp + 4 * i;
+            const int r = row0 + warp + WARPS * i;
             if (r < a.G) {
                 R::template load<false>(q[i], reinterpret_cast<const T*>(a.q) + at.b * a.q_sb + (at.h * a.G + r) * a.q_sh, lane);
             } else {
@@ -240,7 +242,7 @@ template <int D, typename T, int NT> struct QueryRows {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const int r = warp + 4 * i;
+            const int r = warp + WARPS * i;
             R row;
             row.template unpack<T>(q[i]);
             if (a.gamma != nullptr) row.template norm<T>(gamma, a.eps);
@@ -316,7 +318,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
             const int add = min(n - i0, cap - have), count = have + add;
             const int lane = threadIdx.x & 31;
 #pragma unroll 1
-            for (int i = threadIdx.x >> 5; i < add; i += kDecWarps) {
+            for (int i = threadIdx.x >> 5; i < add; i += C::kWarps) {
                 const int cta = from + (i0 + i) * stride;
                 const float* const part = a.ws + decode_part_at<D, E8, NT>(cta, cta == first) + lane * 4;
                 const uint32_t dst = smem_u32(room + (have + i) * size) + lane * 16;
@@ -331,7 +333,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
             i0 += add;
             const float* const m = room + size - 2 * kRows;  // of the first part
 #pragma unroll 1
-            for (int e = threadIdx.x; e < rows * (D / 4); e += kDecThreads) {
+            for (int e = threadIdx.x; e < rows * (D / 4); e += C::kThreads) {
                 const int r = e / (D / 4);
                 float top = -INFINITY, total = 0.f;
 #pragma unroll 4
@@ -420,7 +422,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
 };
 
 template <int D, typename T, bool E8, int NT>
-__global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm) decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E8, NT>::kCtasPerSm) decode_kernel(const DecodeArgs a) {
     using C = DecodeCfg<D, E8, NT>;
     using M = typename std::conditional<E8, __half, T>::type;  // type of the products' operands
     constexpr int kDT = D / 16, kRows = C::kRows;
@@ -488,7 +490,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     auto empty_rows = [&] {  // sequences without rows have no units: their output is zero
         for (int b = blockIdx.x; b < a.B; b += n_ctas)
             if (cached_rows(a, b) == 0)
-                for (int i = tid; i < a.Hkv * a.G * (D / 8); i += kDecThreads)
+                for (int i = tid; i < a.Hkv * a.G * (D / 8); i += C::kThreads)
                     reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
                         make_uint4(0, 0, 0, 0);
     };
@@ -512,11 +514,11 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
     uint4* const frag = reinterpret_cast<uint4*>(smem + C::kRingBytes);
     float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes + C::kQueryBytes);  // two copies of [8][kPad]
     float* const merge_m = merge_o + 2 * 8 * C::kPad;                                        // [warps][rows]
-    float* const merge_l = merge_m + kDecWarps * kRows;
-    float* const back = merge_l + kDecWarps * kRows;                                         // [rows]
+    float* const merge_l = merge_m + C::kWarps * kRows;
+    float* const back = merge_l + C::kWarps * kRows;                                         // [rows]
     unsigned char* const new_rows = smem + C::kSmemBytes - C::kScaleRingBytes - C::kNewBytes;  // K and V row of a new token
 
-    QueryRows<D, T, NT> rows;
+    QueryRows<D, T, NT, C::kWarps> rows;
     using R = Row<D, 32>;
     rows.load(a, cc);
     typename R::Words gamma;
@@ -932,7 +934,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             leave();
         }
 
-        // ---- the four warps' parts of the item together
+        // ---- the warps' parts of the item together
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -954,7 +956,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
             for (int c = 0; c < 2; ++c) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, merge_m[w * kRows + u * 8 + 2 * t4 + c]);
+                for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + u * 8 + 2 * t4 + c]);
                 const float f = mv[u][c] == -INFINITY ? 0.f : ex2(mv[u][c] - (top == -INFINITY ? 0.f : top));
                 // (a warp without keys has a zero output; one whose scores are all -inf keeps a NaN that it may hold)
 #pragma unroll
@@ -967,7 +969,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
         begins_and_goes_on(n);
         float* const part = a.ws + decode_part_at<D, E8, NT>(blockIdx.x, cc.t == 0 ? 1 : 0);
         float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
-        // eight rows and kMergeCols columns at a time: warps 2 and 3 leave theirs, 0 and 1 add theirs, all add the two copies
+        // eight rows and kMergeCols columns at a time: the last two warps leave theirs, two after two add theirs, all add the two copies
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -979,12 +981,15 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                         for (int k = 0; k < 4; ++k)
                             f((2 * t4 + (k & 1)) * C::kPad + 16 * i + (E8 ? 2 * g + (k >> 1) : g + 8 * (k >> 1)), o[u][c0 / 16 + i][k]);
                 };
-                if (warp >= 2) each([&](int at, float x) { copy[at] = x; });
+                if (warp >= C::kWarps - 2) each([&](int at, float x) { copy[at] = x; });
                 __syncthreads();
                 if (u == 0 && c0 == 0 && nc.left > 0) rows.template prepare<E8>(a, gamma, frag, back);  // (all are done with the old ones)
-                if (warp < 2) each([&](int at, float x) { copy[at] += x; });
-                __syncthreads();
-                for (int i = tid; i < 8 * (C::kMergeCols / 4); i += kDecThreads) {
+#pragma unroll 1
+                for (int w = C::kWarps - 4; w >= 0; w -= 2) {
+                    if ((warp & ~1) == w) each([&](int at, float x) { copy[at] += x; });
+                    __syncthreads();
+                }
+                for (int i = tid; i < 8 * (C::kMergeCols / 4); i += C::kThreads) {
                     const int r8 = i / (C::kMergeCols / 4), d8 = (i % (C::kMergeCols / 4)) * 4, r = u * 8 + r8, d = c0 + d8;
                     if (row0 + r >= a.G) break;  // (rows go up with i)
                     const float4 x = *reinterpret_cast<const float4*>(merge_o + r8 * C::kPad + d8);
@@ -992,9 +997,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
                     const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
                     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-                    for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
+                    for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
 #pragma unroll
-                    for (int w = 0; w < kDecWarps; ++w) {
+                    for (int w = 0; w < C::kWarps; ++w) {
                         const float lw = merge_l[w * kRows + r];
                         sum += lw == 0.f ? 0.f : lw * ex2(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
                     }

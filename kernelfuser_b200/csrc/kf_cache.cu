@@ -159,7 +159,7 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
             if (e != cudaSuccess) return fail(KF_ECUDA, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
         }
     }
-    return launched("decode_attention", launch_kernel(kern, dim3(grid), dim3(kf::kDecThreads), smem, st, args));
+    return launched("decode_attention", launch_kernel(kern, dim3(grid), dim3(kf::DecodeCfg<D, E8, NT>::kThreads), smem, st, args));
 }
 
 template <int D, typename T, bool E8> int launch_decode(const kf::DecodeArgs& a, cudaStream_t st) {
