@@ -232,6 +232,48 @@ def test_infinite_scores_give_nan_and_minus_infinite_ones_nothing():
     check(got[1], want[1], bound[1])
 
 
+def test_infinities_in_the_cache_stay_what_they_are():
+    # a value row with +inf or -inf gives that infinity in its column, both give NaN, no other column changes
+    for dtype in (BF, FP):
+        p = Paged([150], 1, 128, 16, dtype, seed=60)
+        q = rand(61, 1, 4, 1, 128, dtype=dtype)
+        clean = kf.decode_attention(q, p.cache, p.pages, ints([150]))
+        at = [(int(p.pages[0, r // 16]), r % 16) for r in (3, 77, 149)]
+        p.v[at[0][0], 0, at[0][1], 5], p.v[at[1][0], 0, at[1][1], 9] = math.inf, -math.inf
+        p.v[at[0][0], 0, at[0][1], 40], p.v[at[2][0], 0, at[2][1], 40] = math.inf, -math.inf
+        got = kf.decode_attention(q, p.cache, p.pages, ints([150]))
+        done()
+        assert (got[..., 5] == math.inf).all() and (got[..., 9] == -math.inf).all() and torch.isnan(got[..., 40]).all()
+        keep = [c for c in range(128) if c not in (5, 9, 40)]
+        assert torch.equal(got[..., keep], clean[..., keep])
+
+
+def test_pools_inside_one_tensor():
+    # K and V pages side by side, [n_pages, 2, Hkv, page, D], as one allocation
+    p = Paged([100, 37], 2, 128, 32, BF, seed=62)
+    both = torch.stack((p.k, p.v), 1)
+    q, new = rand(63, 2, 4, 1, 128), rand(64, 2, 2, 1, 128)
+    got = kf.decode_step(q, new, new, (both[:, 0], both[:, 1]), p.pages, ints([100, 37]))
+    want = kf.decode_step(q, new, new, p.cache, p.pages, ints([100, 37]))
+    done()
+    assert torch.equal(got, want) and torch.equal(both[:, 0], p.k) and torch.equal(both[:, 1], p.v)
+
+
+def test_thousands_of_sequences():
+    lengths = [1 + b % 3 if b % 5 else 0 for b in range(5000)]
+    p = Paged(lengths, 1, 128, 16, BF, seed=65)
+    q = rand(66, 5000, 1, 1, 128)
+    got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+    done()
+    n = torch.tensor(lengths, device="cuda")
+    k, v = (x[p.pages.clamp_min(0).long()[:, 0], 0, :3].double() for x in (p.k, p.v))  # [B, 3, D]
+    s = torch.einsum("bd,bnd->bn", q[:, 0, 0].double(), k) * 128 ** -0.5
+    w = torch.softmax(s.masked_fill(torch.arange(3, device="cuda")[None] >= n[:, None], -math.inf), -1).nan_to_num(0)
+    want = torch.einsum("bn,bnd->bd", w, v)
+    # the output's rounding, and scores off by 2^-16 of |q||k| (about 11.3 of them): p off by 2^-12 of p at most, values below 6
+    assert ((got[:, 0, 0].double() - want).abs() <= want.abs() * U[BF] + 6 * 2.0 ** -11).all()
+
+
 # ---- rows --------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("d,hkv,page,s", [(128, 2, 16, 1), (128, 8, 48, 40), (256, 3, 16, 33), (256, 1, 128, 200)])
