@@ -300,23 +300,29 @@ __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs 
         const unsigned char* const vh = a.c.v + wide(h, a.c.v_sh) + wide(r, a.c.v_ss);
         Raw kx[kReadBlocks], vx[kReadBlocks];
         float kf[kReadBlocks], vf[kReadBlocks];
+        int i = first / a.c.page_size, row = first - i * a.c.page_size;  // page of the sequence and row in it
 #pragma unroll
         for (int u = 0; u < kReadBlocks; ++u) {
             const int s0 = first + u * RPB;
             kx[u] = vx[u] = Raw{};
             kf[u] = vf[u] = 0.f;
             if (s0 >= len) continue;  // (all lanes alike)
-            const int i = s0 / a.c.page_size, row = s0 - i * a.c.page_size, page = __ldg(a.c.pages + b * a.c.pages_sb + i);
+            const int page = __ldg(a.c.pages + b * a.c.pages_sb + i), at = row;
+            row += RPB;
+            if (row >= a.c.page_size) {
+                row = 0;
+                ++i;
+            }
             if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.n_pages)) {
                 report(a.status, kStatusBadPage);
                 continue;
             }
             if (s0 + r >= len) continue;
-            kx[u] = __ldcs(reinterpret_cast<const Raw*>(kh + wide(page, a.c.k_sp) + wide(row, a.c.k_ss)) + sub);
-            vx[u] = __ldcs(reinterpret_cast<const Raw*>(vh + wide(page, a.c.v_sp) + wide(row, a.c.v_ss)) + sub);
+            kx[u] = __ldcs(reinterpret_cast<const Raw*>(kh + wide(page, a.c.k_sp) + wide(at, a.c.k_ss)) + sub);
+            vx[u] = __ldcs(reinterpret_cast<const Raw*>(vh + wide(page, a.c.v_sp) + wide(at, a.c.v_ss)) + sub);
             if constexpr (E8) {
-                kf[u] = scale_value(a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + row + r]);
-                vf[u] = scale_value(a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + row + r]);
+                kf[u] = scale_value(a.c.k_scale[wide(page, a.c.ks_sp) + wide(h, a.c.ks_sh) + at + r]);
+                vf[u] = scale_value(a.c.v_scale[wide(page, a.c.vs_sp) + wide(h, a.c.vs_sh) + at + r]);
             }
         }
         auto put = [&](T* row, const Raw& x, float f) {
@@ -333,13 +339,15 @@ __global__ void __launch_bounds__(kRowsThreads) read_rows_kernel(const ReadArgs 
                 __stcs(reinterpret_cast<uint4*>(row) + sub, x);
             }
         };
-        T* const ko = reinterpret_cast<T*>(a.k) + b * a.k_sb + h * a.k_sh + (first + r) * a.k_ss;
-        T* const vo = reinterpret_cast<T*>(a.v) + b * a.v_sb + h * a.v_sh + (first + r) * a.v_ss;
+        T* ko = reinterpret_cast<T*>(a.k) + b * a.k_sb + h * a.k_sh + (first + r) * a.k_ss;
+        T* vo = reinterpret_cast<T*>(a.v) + b * a.v_sb + h * a.v_sh + (first + r) * a.v_ss;
 #pragma unroll
         for (int u = 0; u < kReadBlocks; ++u) {
             if (first + r + u * RPB >= a.S || failed != 0) continue;
-            put(ko + u * RPB * a.k_ss, kx[u], kf[u]);
-            put(vo + u * RPB * a.v_ss, vx[u], vf[u]);
+            put(ko, kx[u], kf[u]);
+            put(vo, vx[u], vf[u]);
+            ko += RPB * a.k_ss;
+            vo += RPB * a.v_ss;
         }
     }
 }
