@@ -55,7 +55,7 @@ struct DecodeArgs {
 
 // Items of up to this many units are not broken for CTAs that would be idle: joining costs about as much as four units of one
 // warp each (3 units: 8.7 us whole, 9.7 broken).  Longer ones are, down to single units (128 units 17.8 -> 14.8 us, 16: 13.4 -> 11.4).
-constexpr int kDecWhole = 4;
+constexpr int kDecWhole = 4;  // (of 64 keys of 128; wider or longer units take that much longer)
 
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         }
         const unsigned int sum = __shfl_sync(0xffffffffu, before, 31), total = sum * HK;  // (the host has seen to it that this fits)
         const unsigned int average = sum / max(__reduce_add_sync(0xffffffffu, rows_at_all), 1u);
-        const unsigned int least = average <= kDecWhole + C::kItemCost ? average : 1 + C::kItemCost;
+        const unsigned int least = average <= kDecWhole / (C::kTiles * (D / 128)) + C::kItemCost ? average : 1 + C::kItemCost;
         piece = max((total + n_ctas - 1) / n_ctas, max(least, 1u));
         u0 = piece * blockIdx.x;
         u1 = min(u0 + piece, total);
