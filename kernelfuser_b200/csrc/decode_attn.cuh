@@ -773,8 +773,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                         if constexpr (kSplit) mma16816<M>(s[u][tile][1], a0, a1, a2, a3, f.z, f.w);
                     }
                 };
-                float scale = 1.f;  // of key `lane` of the step
-                if constexpr (E8) scale = scale_value(scales[slot * C::kKeys + lane]);
+                float scale = 1.f;  // of key `lane` of the step (with steps of 16 keys, twice)
+                if constexpr (E8) scale = scale_value(scales[slot * C::kKeys + lane % C::kKeys]);
                 const uint32_t k_at = k_lane + slot * C::kSlotBytes;
 #pragma unroll
                 for (int j = 0; j < kDT; j += E8 ? 2 : 1)
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                 bool above = false;
                 if constexpr (E8) {
                     // exponent of value row `lane` of the step (2^23 + e as bits: e - 127 without a conversion)
-                    const uint32_t e = scales[slot * C::kKeys + lane];
+                    const uint32_t e = scales[slot * C::kKeys + lane % C::kKeys];
                     const float exponent = e == 255 ? NAN : __uint_as_float(0x4b000000u | e) - 8388735.f;
 #pragma unroll
                     for (int tile = 0; tile < C::kTiles; ++tile) {

@@ -64,8 +64,10 @@ EDGE = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 0, 127, 128, 129, 255, 257, -3, 30
     (128, 3, 3, 48, False, True),    # heads without sharing, pages that are no power of two
     (128, 12, 1, 32, True, False),   # two n8 blocks, the second half full
     (128, 40, 2, 64, True, True),    # two blocks of 16 rows, the second one short
+    (128, 35, 1, 16, False, True),   # three blocks
     (256, 4, 2, 16, True, True),
     (256, 11, 1, 80, False, False),
+    (256, 17, 1, 16, True, True),    # a block of 16 rows and a single one
 ])
 def test_attention_at_edge_lengths(cache, dtype, d, hq, hkv, page, norm, rope):
     p = Paged(EDGE, hkv, d, page, E8 if cache == "e4m3" else dtype, seed=1, max_pages=20)
@@ -89,6 +91,11 @@ def test_attention_at_edge_lengths(cache, dtype, d, hq, hkv, page, norm, rope):
     ([9000, 1, 0, 5000, 13], 4, 2, 128),  # broken items next to whole ones
     ([20000, 64], 2, 1, 256),
     ([4097] * 3, 16, 1, 256),
+    ([6000, 700], 24, 1, 128),
+    ([900] * 150, 24, 1, 128),            # whole items of many units: every slot of a ring is used, again and again
+    ([1500] * 150, 16, 1, 256),
+    ([1300] * 300, 2, 1, 256),
+    ([2100] * 450, 3, 1, 128),
     ([900] * 40, 8, 4, 128),
 ])
 def test_long_sequences_are_split_and_joined(cache, lengths, hq, hkv, d):
