@@ -181,7 +181,8 @@ def append_rows(cache, k, v, pages, start, gk=None, cos=None, sin=None, *, count
               0 if sin is None else sin.data_ptr(), start.data_ptr(), 0 if counts is None else counts.data_ptr(),
               _status_ptr(index), b, s, _DTYPES[k.dtype], n_pos)
     with _on_device(index):
-        _call(_lib.load().kf_append_rows(_APPEND.pack(*fields, *packed, *k.stride()[:3], *v.stride()[:3], eps), _raw_stream(index)))
+        params = _APPEND.pack(*fields, *packed, *k.stride()[:3], *v.stride()[:3], eps)
+        _call(_lib.load().kf_append_rows(params, _raw_stream(index)))
     return cache
 
 

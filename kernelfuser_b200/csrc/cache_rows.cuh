@@ -7,7 +7,8 @@
 // holds a row as e4m3 values times ONE power of two, kept as its exponent byte (e8m0): the smallest that brings the
 // row's largest magnitude to at most 448.  A power of two costs no precision that e4m3 has (only its subnormals begin
 // up to a factor of two earlier) and makes scaling exact, so that each value is rounded once and reading back to 16
-// bits is exact.  (Magnitudes above 448 * 2^119 = 2.98e38 become that.)  A row whose largest magnitude is not finite gets the NaN scale and reads back as NaN.
+// bits is exact.  (Magnitudes above 448 * 2^119 = 2.98e38 become that.)  A row whose largest magnitude is not finite
+// gets the NaN scale and reads back as NaN.
 #pragma once
 #include <type_traits>
 
@@ -189,10 +190,10 @@ struct AppendArgs {
 
 constexpr int kRowsThreads = 256;
 
-// A group of D/16 lanes takes up to kAppendHeads heads of one position, so that the tables are read once for them and their rows
-// are in flight together; K rows and V rows are different CTAs' work (blockIdx.z).  Bound by HBM (16 bits: 16384 rows of
-// eight heads in 26.7 us = 5.06 TB/s; one head in flight 33, K and V in one lane 43) and by the latency of a CTA's chain of
-// loads: 80 registers, three CTAs an SM (e4m3 30.5 -> 26.7 us).
+// A group of D/16 lanes takes up to kAppendHeads heads of one position, so that the tables are read once for them and their
+// rows are in flight together; K rows and V rows are different CTAs' work (blockIdx.z).  Bound by HBM (16 bits: 16384 rows
+// of eight heads in 26.5 us = 5.1 TB/s; one head in flight 33, K and V in one lane 43) and by the latency of a CTA's chain
+// of loads: 80 registers, three CTAs an SM (e4m3 30.5 -> 26.7 us).
 constexpr int kAppendHeads = 4;
 
 template <int D, typename T, bool E8>
@@ -250,7 +251,8 @@ __global__ void __launch_bounds__(kRowsThreads, 3) append_rows_kernel(const Appe
                               : a.c.v + wide(page, a.c.v_sp) + wide(row, a.c.v_ss) + wide(h0, a.c.v_sh);
     unsigned char* scale = nullptr;
     if constexpr (E8)
-        scale = is_k ? a.c.k_scale + wide(page, a.c.ks_sp) + wide(h0, a.c.ks_sh) + row : a.c.v_scale + wide(page, a.c.vs_sp) + wide(h0, a.c.vs_sh) + row;
+        scale = is_k ? a.c.k_scale + wide(page, a.c.ks_sp) + wide(h0, a.c.ks_sh) + row
+                     : a.c.v_scale + wide(page, a.c.vs_sp) + wide(h0, a.c.vs_sh) + row;
     const int dst_h = is_k ? a.c.k_sh : a.c.v_sh, scale_h = is_k ? a.c.ks_sh : a.c.vs_sh;
 #pragma unroll
     for (int i = 0; i < kAppendHeads; ++i) {

@@ -6,21 +6,23 @@
 // What bounds it.  Every cached byte is read once and serves G query heads: 4 D G operations per 4 D bytes of a 16-bit
 // cache, a few operations a byte, so HBM sets the time and everything else has to stay out of its way.
 //
-// Work split.  The unit of work is 64 keys of one (sequence, KV head), or 128 of an 8-bit cache.  All units of the launch are laid in one line and
-// every CTA takes an equal piece of it, found from the lengths on the device: ragged batches and single long sequences
-// load all SMs alike, and a captured launch follows its lengths.  A CTA's piece covers whole (sequence, head) items and
-// at most two broken ones; a broken item's parts meet in the workspace, where the CTA that comes last joins them, in the
-// order of the line whoever that is: as many at a time as its ring holds, and if there are more, the joined groups once more.  (A second kernel
-// for it cost 2 us of a call, and its serial pass over 37 parts of a long sequence 12 us.)
+// Work split.  The unit of work is 64 keys of one (sequence, KV head), 128 where a warp's step is 32 keys or a CTA has
+// eight warps.  All units of the launch are laid in one line and every CTA takes an equal piece of it, found from the
+// lengths on the device: ragged batches and single long sequences load all SMs alike, and a captured launch follows its
+// lengths.  A CTA's piece covers whole (sequence, head) items and at most two broken ones; a broken item's parts meet in
+// the workspace, where the CTA that comes last joins them, in the order of the line whoever that is: as many at a time as
+// its ring holds, and if there are more, the joined groups once more.  (A second kernel for it cost 2 us of a call, and
+// its serial pass over 37 parts of a long sequence 12 us.)
 //
-// Inside a CTA each of the four (or eight) warps is a stream of its own: of every unit it takes 16 keys, copies their K and V rows
-// into its own ring of slots in shared memory (cp.async, across item borders), and keeps its own sum and output; they
-// meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are the m16 of mma.m16n8k16 and the
-// query heads its n8, so up to eight heads cost one instruction per 16 x 16 block of the cache.  (The 128-row MMAs of the
-// prefill kernels have nothing to fill their rows with here.)  Q is prepared once per item, a row to a warp, from values
-// that are loaded while the item before is computed.
-// The exponentials are taken against a base that is only moved when a score exceeds it by more than 2^8 (exact after the
-// division by the sum): as a rule no lane waits for a maximum over lanes.
+// Inside a CTA each of the four (or eight) warps is a stream of its own: of every unit it takes a step of 16 keys (32 of an
+// 8-bit cache), copies their K and V rows into its own ring of slots in shared memory (cp.async, across item borders), and
+// keeps its own sum and output; they meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are
+// the m16 of mma.m16n8k16 and the query heads its n8, so up to eight heads cost one instruction per 16 x 16 block of the
+// cache.  (The 128-row MMAs of the prefill kernels have nothing to fill their rows with here.)  Q is prepared once per item,
+// a row to a warp, from values that are loaded while the item before is computed.
+// The exponentials are taken against a base that is only moved when a score exceeds it by more than a factor of 2^8 (2^4
+// where probabilities enter in f16), which is exact after the division by the sum: as a rule no lane waits for a maximum
+// over lanes.
 // A new token's K and V rows are prepared by the warp that has their step, which puts them into the cache and, for itself,
 // behind the step's cached rows in shared memory: nobody else reads them, so nobody has to wait.
 // Rounding: q' and the probabilities enter the products as the sum of two 16-bit numbers, so that what is left of them is
@@ -53,15 +55,16 @@ struct DecodeArgs {
     int* status;
 };
 
-// Items of up to this many units are not broken for CTAs that would be idle: joining costs about as much as four units of one
-// warp each (3 units: 8.7 us whole, 9.7 broken).  Longer ones are, down to single units (128 units 17.8 -> 14.8 us, 16: 13.4 -> 11.4).
+// Items of up to this many units are not broken for CTAs that would be idle: joining costs about as much as four units (3
+// units: 8.7 us whole, 9.7 broken).  Longer ones are, down to single units (128 units 17.8 -> 14.8 us, 16: 13.4 -> 11.4).
 constexpr int kDecWhole = 4;  // (of 64 keys of 128; wider or longer units take that much longer)
 
 template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kRows = 8 * NT;
     static constexpr bool kWide = D == 256 && NT == 2;                // more than eight heads of 256
     static constexpr int kWarps = kWide ? 8 : 4, kThreads = 32 * kWarps;
-    static constexpr int kTiles = E8 && !kWide ? 2 : 1, kKeys = 16 * kTiles, kUnit = kKeys * kWarps;  // keys of a warp's step, of a unit
+    static constexpr int kTiles = E8 && !kWide ? 2 : 1, kKeys = 16 * kTiles;  // blocks of 16 keys, keys of a warp's step
+    static constexpr int kUnit = kKeys * kWarps;
     static constexpr int kRowBytes = D * (E8 ? 1 : 2);
     // What an item costs beside its units, in units of its keys: about 3 us of a CTA (looking up its rows, preparing its
     // queries, meeting of the warps), which hold a unit of 64 KB or two of 32.  32 ragged sequences of up to 1500 rows: 1 -> 36
@@ -77,7 +80,8 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     // With more than eight heads of 256 O alone takes 128 registers and one CTA's queries 16 KB: eight warps share them.
     // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
     static constexpr int kSlots = E8 ? (kWide || (D == 128 && NT == 2) ? 5 : 3) : D == 256 ? 3 : NT == 1 ? 6 : 5;
-    static constexpr int kMergeCols = D == 256 || E8 ? 64 : 128, kPad = kMergeCols + 4;  // columns that meet at a time; a row in shared memory
+    // columns that meet at a time; a row of them in shared memory
+    static constexpr int kMergeCols = D == 256 || E8 ? 64 : 128, kPad = kMergeCols + 4;
     static constexpr int kRingBytes = kWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
@@ -103,8 +107,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int DST, int SRC> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "l"(policy), "n"(DST), "n"(SRC)
-                 : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "l"(policy),
+                 "n"(DST), "n"(SRC) : "memory");
 }
 template <typename F, int... I> __device__ __forceinline__ void each_index(F&& f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
@@ -144,7 +148,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-__device__ __forceinline__ int cached_rows(const DecodeArgs& a, int b) { return min(max(__ldg(a.lengths + b), 0), a.c.capacity); }
+__device__ __forceinline__ int cached_rows(const DecodeArgs& a, int b) {
+    return min(max(__ldg(a.lengths + b), 0), a.c.capacity);
+}
 template <int UNIT> __device__ __forceinline__ int units_of(int len) { return (len + UNIT - 1) / UNIT; }
 
 // A place in the line of units: unit t of nt of item hk of sequence b.
@@ -199,7 +205,8 @@ template <typename M> __device__ __forceinline__ void split2(float x, float y, u
     low = Num<M>::pack(rest(x, h.x), rest(y, h.y));
 }
 // probabilities; FLOOR: against infinities in the cache (an 8-bit one has none)
-template <typename M, bool FLOOR> __device__ __forceinline__ void split2_probabilities(float x, float y, uint32_t& high, uint32_t& low) {
+template <typename M, bool FLOOR>
+__device__ __forceinline__ void split2_probabilities(float x, float y, uint32_t& high, uint32_t& low) {
     if constexpr (FLOOR) {  // (x < kMin and not max(): a NaN stays one)
         x = x < Split<M>::kMin ? Split<M>::kMin : x;
         y = y < Split<M>::kMin ? Split<M>::kMin : y;
@@ -237,7 +244,8 @@ template <int D, typename T, int NT, int WARPS> struct QueryRows {
     // Norm, rotation, and the fragments of the products into shared memory: lane l of a fragment holds row l/4, and of 16
     // columns 2t, 2t+1, 2t+8, 2t+9 (16-bit cache) or 4t .. 4t+3 (8-bit), t = l%4, as a K fragment of that step does.
     // back[row]: what the row's scores are to be multiplied with to undo the scaling of its values (8-bit cache).
-    template <bool E8> __device__ __forceinline__ void prepare(const DecodeArgs& a, const typename R::Words& gamma, uint4* frag, float* back) const {
+    template <bool E8>
+    __device__ __forceinline__ void prepare(const DecodeArgs& a, const typename R::Words& gamma, uint4* frag, float* back) const {
         using M = typename std::conditional<E8, __half, T>::type;
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -353,7 +361,8 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                 } else {
                     const float inv = 1.f / total;
                     T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + e % (D / 4) * 4;
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+                    *reinterpret_cast<uint2*>(dst) =
+                        make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
                 }
             }
             if (i0 >= n && out == nullptr) break;
@@ -385,7 +394,8 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
             const DecodeBroken& it = item[threadIdx.x / 32];
             bool all = false;
             if (it.first >= 0) {
-                const int group = join_group(it.last - it.first + 1), from = it.first + (cta - it.first) / group * group, n = min(group, it.last - from + 1);
+                const int group = join_group(it.last - it.first + 1);
+                const int from = it.first + (cta - it.first) / group * group, n = min(group, it.last - from + 1);
                 all = n == 1 || count_up(from, from == it.first ? 8 : 0, n);
             }
             __threadfence();
@@ -396,7 +406,8 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
         for (int k = 0; k < 2; ++k) {
             if (s_flag[k] == 0) continue;
             const DecodeBroken it = k == 0 ? item[0] : item[1];
-            const int group = join_group(it.last - it.first + 1), groups = (it.last - it.first) / group + 1, row0 = (it.hk - it.h * a.row_blocks) * kRows;
+            const int group = join_group(it.last - it.first + 1), groups = (it.last - it.first) / group + 1;
+            const int row0 = (it.hk - it.h * a.row_blocks) * kRows;
             int from = it.first + (cta - it.first) / group * group, stride = 1, n = min(group, it.last - from + 1);
             bool final = groups == 1;
 #pragma unroll 1
@@ -422,7 +433,8 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
 };
 
 template <int D, typename T, bool E8, int NT>
-__global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E8, NT>::kCtasPerSm) decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E8, NT>::kCtasPerSm)
+    decode_kernel(const DecodeArgs a) {
     using C = DecodeCfg<D, E8, NT>;
     using M = typename std::conditional<E8, __half, T>::type;  // type of the products' operands
     constexpr int kDT = D / 16, kRows = C::kRows;
@@ -501,9 +513,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     }
     // the broken items: the one that began before this piece (or fills it), and the one that begins in it and goes on
     DecodeBroken broken[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};
-    if (cc.t > 0) broken[0] = {static_cast<int>((u1 - cc.left - cc.t) / piece), static_cast<int>((u1 - cc.left - cc.t + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
+    auto cta_of = [&](unsigned int u) { return static_cast<int>(u / piece); };
+    if (cc.t > 0) {
+        const unsigned int from = u1 - cc.left - cc.t;  // the item's first unit
+        broken[0] = {cta_of(from), cta_of(from + cc.nt - 1), cc.b, cc.hk, cc.h};
+    }
     auto begins_and_goes_on = [&](int n) {  // n units of item cc are here
-        if (cc.t == 0 && n < cc.nt) broken[1] = {static_cast<int>(blockIdx.x), static_cast<int>((u1 - cc.left + cc.nt - 1) / piece), cc.b, cc.hk, cc.h};
+        if (cc.t == 0 && n < cc.nt)
+            broken[1] = {static_cast<int>(blockIdx.x), cta_of(u1 - cc.left + cc.nt - 1), cc.b, cc.hk, cc.h};
     };
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
@@ -526,7 +543,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
 
     auto pc = cc;
     constexpr int kLook = 32 / C::kTiles;        // units whose pages the lanes hold
-    int table_at = 0, my_page = 0, my_row = 0;  // lane i: page and row in it of the warp's 16 keys i of the units from table_at on
+    // lane i: page and row in it of the warp's i-th 16 keys of the units from table_at on
+    int table_at = 0, my_page = 0, my_row = 0;
     int page[C::kTiles] = {}, page_row[C::kTiles] = {};  // of the unit that is being copied
     constexpr int kPieces = C::kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kCopies = 16 / kRowsAtOnce;
     const int piece16 = lane % kPieces, r_lane = lane / kPieces;
@@ -568,7 +586,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             }
             if constexpr (E8) {  // (all 16 scales: a page holds a multiple of 16 rows)
                 if (lane == 0)
-                    cp_async16<0, 0>(smem_u32(scales) + slot * C::kKeys + 16 * tile, scale + wide(page[tile], scale_sp) + page_row[tile], policy);
+                    cp_async16<0, 0>(smem_u32(scales) + slot * C::kKeys + 16 * tile,
+                                     scale + wide(page[tile], scale_sp) + page_row[tile], policy);
             }
         }
     };
@@ -667,7 +686,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             R::template load<false>(c, reinterpret_cast<const T*>(a.cos) + at, lane);
             R::template load<false>(s, reinterpret_cast<const T*>(a.sin) + at, lane);
         }
-        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) write = false;  // (reported by the copies of the step)
+        // (reported by the copies of the step)
+        if (static_cast<unsigned>(pg) >= static_cast<unsigned>(a.c.n_pages)) write = false;
         R k, v;
         k.template unpack<T>(kw);
         v.template unpack<T>(vw);
@@ -680,8 +700,10 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             };
         };
         const int p = write ? pg : 0;
-        new_ke = k.template store<T, E8>(lane, to(new_rows, a.c.k + wide(p, a.c.k_sp) + wide(cc.h, a.c.k_sh) + wide(row, a.c.k_ss)));
-        new_ve = v.template store<T, E8>(lane, to(new_rows + C::kRowBytes, a.c.v + wide(p, a.c.v_sp) + wide(cc.h, a.c.v_sh) + wide(row, a.c.v_ss)));
+        unsigned char* const k_to = a.c.k + wide(p, a.c.k_sp) + wide(cc.h, a.c.k_sh) + wide(row, a.c.k_ss);
+        unsigned char* const v_to = a.c.v + wide(p, a.c.v_sp) + wide(cc.h, a.c.v_sh) + wide(row, a.c.v_ss);
+        new_ke = k.template store<T, E8>(lane, to(new_rows, k_to));
+        new_ve = v.template store<T, E8>(lane, to(new_rows + C::kRowBytes, v_to));
         if (E8 && write && lane == 0) {
             a.c.k_scale[wide(p, a.c.ks_sp) + wide(cc.h, a.c.ks_sh) + row] = static_cast<unsigned char>(new_ke);
             a.c.v_scale[wide(p, a.c.vs_sp) + wide(cc.h, a.c.vs_sh) + row] = static_cast<unsigned char>(new_ve);
@@ -768,7 +790,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                 auto product = [&](int tile, int j, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                     for (int u = 0; u < NT; ++u) {
-                        const uint4 f = C::kQueryInRegs ? qf[C::kQueryInRegs ? u : 0][C::kQueryInRegs ? j : 0] : frag[(u * kDT + j) * 32 + lane];
+                        uint4 f;
+                        if constexpr (C::kQueryInRegs) f = qf[u][j];
+                        else f = frag[(u * kDT + j) * 32 + lane];
                         mma16816<M>(s[u][tile][0], a0, a1, a2, a3, f.x, f.y);
                         if constexpr (kSplit) mma16816<M>(s[u][tile][1], a0, a1, a2, a3, f.z, f.w);
                     }
@@ -828,7 +852,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                     const float exponent = e == 255 ? NAN : __uint_as_float(0x4b000000u | e) - 8388735.f;
 #pragma unroll
                     for (int tile = 0; tile < C::kTiles; ++tile) {
-                        const float ve0 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g), ve1 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g + 8);
+                        const float ve0 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g);
+                        const float ve1 = __shfl_sync(0xffffffffu, exponent, 16 * tile + g + 8);
 #pragma unroll
                         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -969,7 +994,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         begins_and_goes_on(n);
         float* const part = a.ws + decode_part_at<D, E8, NT>(blockIdx.x, cc.t == 0 ? 1 : 0);
         float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
-        // eight rows and kMergeCols columns at a time: the last two warps leave theirs, two after two add theirs, all add the two copies
+        // eight rows and kMergeCols columns at a time: the last two warps leave theirs, two after two add theirs, all add the
+        // two copies
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -979,11 +1005,13 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                     for (int i = 0; i < C::kMergeCols / 16; ++i)
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            f((2 * t4 + (k & 1)) * C::kPad + 16 * i + (E8 ? 2 * g + (k >> 1) : g + 8 * (k >> 1)), o[u][c0 / 16 + i][k]);
+                            f((2 * t4 + (k & 1)) * C::kPad + 16 * i + (E8 ? 2 * g + (k >> 1) : g + 8 * (k >> 1)),
+                              o[u][c0 / 16 + i][k]);
                 };
                 if (warp >= C::kWarps - 2) each([&](int at, float x) { copy[at] = x; });
                 __syncthreads();
-                if (u == 0 && c0 == 0 && nc.left > 0) rows.template prepare<E8>(a, gamma, frag, back);  // (all are done with the old ones)
+                // (all are done with the old ones)
+                if (u == 0 && c0 == 0 && nc.left > 0) rows.template prepare<E8>(a, gamma, frag, back);
 #pragma unroll 1
                 for (int w = C::kWarps - 4; w >= 0; w -= 2) {
                     if ((warp & ~1) == w) each([&](int at, float x) { copy[at] += x; });
@@ -1006,7 +1034,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                     if (whole) {
                         T* const dst = reinterpret_cast<T*>(a.out) + cc.b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
                         const float inv = 1.f / sum;
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+                        *reinterpret_cast<uint2*>(dst) =
+                            make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
                     } else {
                         *reinterpret_cast<float4*>(part + r * D + d) = z;
                         if (d == 0) {

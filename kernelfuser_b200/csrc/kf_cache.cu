@@ -33,7 +33,8 @@ int cache_view(const kf_paged_cache& c, int64_t dtype, kf::CacheView* out) {
     if (!aligned16(c.k) || !aligned16(c.v)) return fail(KF_EALIGN, "pointers must be 16-byte aligned");
     const bool e8 = c.dtype == KF_E4M3;
     const int64_t step = e8 ? 16 : 8, size = e8 ? 1 : 2;
-    const int64_t strides[6] = {c.k_stride_page, c.k_stride_head, c.k_stride_row, c.v_stride_page, c.v_stride_head, c.v_stride_row};
+    const int64_t strides[6] = {c.k_stride_page, c.k_stride_head, c.k_stride_row,
+                                c.v_stride_page, c.v_stride_head, c.v_stride_row};
     const int64_t extents[3] = {c.n_pages, c.Hkv, c.page_size};
     for (int i = 0; i < 6; ++i)
         if (!step_ok(strides[i], extents[i % 3], step))
@@ -73,7 +74,8 @@ int cache_view(const kf_paged_cache& c, int64_t dtype, kf::CacheView* out) {
     return KF_OK;
 }
 
-int check_rows(const char* what, const void* p, int64_t B, int64_t H, int64_t S, int64_t D, int64_t sb, int64_t sh, int64_t ss) {
+int check_rows(const char* what, const void* p, int64_t B, int64_t H, int64_t S, int64_t D, int64_t sb, int64_t sh,
+               int64_t ss) {
     if (!p) return fail(KF_EINVAL, "%s must not be NULL", what);
     if (!aligned16(p)) return fail(KF_EALIGN, "pointers must be 16-byte aligned");
     if (!step_ok(sb, B, 8) || !step_ok(sh, H, 8) || !step_ok(ss, S, 8))
@@ -84,7 +86,8 @@ int check_rows(const char* what, const void* p, int64_t B, int64_t H, int64_t S,
 
 int check_tables(const void* gamma, const void* cos_table, const void* sin_table, int64_t n_positions) {
     if ((cos_table == nullptr) != (sin_table == nullptr)) return fail(KF_EINVAL, "provide both rotary tables or neither");
-    if (!aligned16(gamma) || !aligned16(cos_table) || !aligned16(sin_table)) return fail(KF_EALIGN, "pointers must be 16-byte aligned");
+    if (!aligned16(gamma) || !aligned16(cos_table) || !aligned16(sin_table))
+        return fail(KF_EALIGN, "pointers must be 16-byte aligned");
     if (cos_table) return check_sizes("n_positions", n_positions, 0x7fffffff);
     return KF_OK;
 }
@@ -102,7 +105,8 @@ template <int D, typename T, bool E8> int launch_append(const kf::AppendArgs& a,
     args.heads_per_group = gx * ((a.H + kf::kAppendHeads - 1) / kf::kAppendHeads) >= sm_count() ? kf::kAppendHeads : 1;
     const unsigned gy = (unsigned)((a.H + args.heads_per_group - 1) / args.heads_per_group);
     if (gy > 65535) return fail(KF_EINVAL, "too many heads");
-    return launched("append_rows", launch_kernel(kf::append_rows_kernel<D, T, E8>, dim3((unsigned)gx, gy, 2), dim3(kf::kRowsThreads), 0, st, args));
+    return launched("append_rows", launch_kernel(kf::append_rows_kernel<D, T, E8>, dim3((unsigned)gx, gy, 2),
+                                                 dim3(kf::kRowsThreads), 0, st, args));
 }
 
 template <int D, typename T, bool E8> int launch_read(const kf::ReadArgs& a, cudaStream_t st) {
@@ -146,9 +150,11 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     kf::DecodeArgs args = a;
     args.row_blocks = (a.G + 8 * NT - 1) / (8 * NT);
     // no more CTAs than the batch can have pieces of work
-    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, unit = kf::DecodeCfg<D, E8, NT>::kUnit, per_item = (a.c.capacity + unit - 1) / unit;
+    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, unit = kf::DecodeCfg<D, E8, NT>::kUnit;
+    const long long per_item = (a.c.capacity + unit - 1) / unit;
     const long long most = items * (per_item + kf::DecodeCfg<D, E8, NT>::kItemCost);
-    if (most > 0x7fffffffLL) return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
+    if (most > 0x7fffffffLL)
+        return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
     const long long fit = decode_ctas<D, E8, NT>();
     const unsigned grid = (unsigned)(items * per_item < fit ? items * per_item : fit);
     if (grid > 1) {
@@ -159,7 +165,8 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
             if (e != cudaSuccess) return fail(KF_ECUDA, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
         }
     }
-    return launched("decode_attention", launch_kernel(kern, dim3(grid), dim3(kf::DecodeCfg<D, E8, NT>::kThreads), smem, st, args));
+    return launched("decode_attention",
+                    launch_kernel(kern, dim3(grid), dim3(kf::DecodeCfg<D, E8, NT>::kThreads), smem, st, args));
 }
 
 template <int D, typename T, bool E8> int launch_decode(const kf::DecodeArgs& a, cudaStream_t st) {
