@@ -310,9 +310,13 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
 
     static constexpr int kQuads = kRows * (D / 4) / C::kThreads;  // groups of four columns that a thread sums up, at most
 
-    // One thread: count one more in the field; true for the CTA that completes `count`.
+    // One thread: count one more in the field; true for the CTA that completes `count`.  What the CTA has written before a
+    // barrier in front of this is visible to whoever counts later, behind a barrier of theirs.  (acq_rel: with full fences
+    // around a plain atomic the 16 sequences below take 28.1 instead of 26.6 us, the smallest broken calls 0.4 more.)
     __device__ __forceinline__ bool count_up(int cta, int shift, int count) const {
-        const unsigned int before = atomicAdd(a.arrived + cta, 1u << shift);
+        unsigned int before;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(before)
+                     : "l"(a.arrived + cta), "r"(1u << shift) : "memory");
         const bool all = static_cast<int>(before >> shift & (shift == 16 ? 0xffffu : 0xffu)) == count - 1;
         if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
         return all;
@@ -399,10 +403,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
         const int group = join_group(it.last - it.first + 1);
         const int from = it.first + (static_cast<int>(blockIdx.x) - it.first) / group * group;
         const int n = min(group, it.last - from + 1);
-        __threadfence();  // the part is visible before it counts
-        const bool all = n == 1 || count_up(from, from == it.first ? 8 : 0, n);
-        __threadfence();
-        return all;
+        return n == 1 || count_up(from, from == it.first ? 8 : 0, n);
     }
     // All threads, once, behind the counting: the joins that fall to this CTA (those whose s_flag is set).
     __device__ __forceinline__ void run(const DecodeBroken (&item)[2], bool dead) const {
@@ -421,11 +422,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                 if (n > 1 && !dead) sum(it.first, from, stride, n, place, it.b, it.h, row0);
                 if (final) break;
                 __syncthreads();
-                if (threadIdx.x == 0) {
-                    __threadfence();
-                    s_flag[k] = count_up(it.first, 16, groups);
-                    __threadfence();
-                }
+                if (threadIdx.x == 0) s_flag[k] = count_up(it.first, 16, groups);
                 __syncthreads();
                 if (s_flag[k] == 0) break;
                 from = it.first;
