@@ -14,6 +14,10 @@
 // its ring holds, and if there are more, the joined groups once more.  (A second kernel for it cost 2 us of a call, and
 // its serial pass over 37 parts of a long sequence 12 us.)
 //
+// More than sixteen query heads of a KV head are blocks of sixteen, a CTA each for the same piece of the line: they run side
+// by side, so that HBM gives a row to one of them and L2 to the others (128 sequences of 8192 rows, 24 heads: 173 us when
+// the blocks were items one behind the other, 148; 48/2 heads of 256, 32 sequences: 176 -> 132).
+//
 // Inside a CTA each of the four (or eight) warps is a stream of its own: of every unit it takes a step of 16 keys (32 of an
 // 8-bit cache), copies their K and V rows into its own ring of slots in shared memory (cp.async, across item borders), and
 // keeps its own sum and output; they meet once per item.  S^T = K Q^T and O^T = V^T P^T: the 16 keys (16 columns of V) are
@@ -153,19 +157,17 @@ __device__ __forceinline__ int cached_rows(const DecodeArgs& a, int b) {
 }
 template <int UNIT> __device__ __forceinline__ int units_of(int len) { return (len + UNIT - 1) / UNIT; }
 
-// A place in the line of units: unit t of nt of item hk of sequence b.
+// A place in the line of units: unit t of nt of KV head h of sequence b.
 template <int UNIT, int COST> struct DecodeCursor {
-    int b, hk, h, t, nt, len;
+    int b, h, t, nt, len;
     int left;  // of the line up to the end of the CTA's piece
     // to the next item, if the piece reaches it
-    __device__ __forceinline__ void next_item(const DecodeArgs& a, int HK) {
+    __device__ __forceinline__ void next_item(const DecodeArgs& a) {
         left -= COST;
         if (left <= 0) return;
         t = 0;
-        ++hk;
-        h = hk / a.row_blocks;
-        if (hk < HK) return;
-        hk = h = 0;
+        if (++h < a.Hkv) return;
+        h = 0;
         do len = cached_rows(a, ++b); while (len == 0 && b + 1 < a.B);
         nt = units_of<UNIT>(len);
     }
@@ -223,8 +225,8 @@ template <int D, typename T, int NT, int WARPS> struct QueryRows {
     using R = Row<D, 32>;
     static constexpr int kN = 8 * NT / WARPS;  // rows of a warp
     typename R::Words q[kN], cos, sin;
-    template <typename Cursor> __device__ __forceinline__ void load(const DecodeArgs& a, const Cursor& at) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row0 = (at.hk - at.h * a.row_blocks) * 8 * NT;
+    template <typename Cursor> __device__ __forceinline__ void load(const DecodeArgs& a, const Cursor& at, int row0) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const int r = row0 + warp + WARPS * i;
@@ -285,12 +287,13 @@ template <int D, bool E8, int NT> __host__ __device__ constexpr long long decode
     return decode_part_at<D, E8, NT>(ctas, 0) + ctas;
 }
 
-// Joining.  Item parts of CTAs first .. last (one that begins in `first`); groups of join_group() consecutive ones.  A CTA's
-// word counts in three fields: parts that have arrived of the group whose first part is its part 0 (bits 0-7) or its part 1
-// (8-15), and joined groups of the item that begins in it (16-31).  Who completes a field takes it back to zero.
+// Joining.  CTAs are numbered here among those of one block of query rows.  Item parts of CTAs first .. last (one that begins
+// in `first`); groups of join_group() consecutive ones.  A CTA's word counts in three fields: parts that have arrived of the
+// group whose first part is its part 0 (bits 0-7) or its part 1 (8-15), and joined groups of the item that begins in it
+// (16-31).  Who completes a field takes it back to zero.
 struct DecodeBroken {
     int first, last;  // its CTAs; first < 0: there is none
-    int b, hk, h;
+    int b, h;
 };
 
 template <int D, typename T, bool E8, int NT> struct DecodeJoin {
@@ -299,6 +302,13 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     const DecodeArgs& a;
     float* room;     // shared memory: the ring
     int* s_flag;     // shared memory: 2
+    int cta, row_block;
+
+    __device__ __forceinline__ int row0() const { return row_block * kRows; }
+    __device__ __forceinline__ int index(int of) const { return of * a.row_blocks + row_block; }  // in the grid
+    __device__ __forceinline__ float* part(int of, bool begins) const {
+        return a.ws + decode_part_at<D, E8, NT>(index(of), begins);
+    }
 
     // parts that the ring holds side by side, of rows that exist
     __device__ __forceinline__ int part_floats() const { return min(kRows, a.G) * D + 2 * kRows; }
@@ -313,19 +323,19 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     // One thread: count one more in the field; true for the CTA that completes `count`.  What the CTA has written before a
     // barrier in front of this is visible to whoever counts later, behind a barrier of theirs.  (acq_rel: with full fences
     // around a plain atomic the 16 sequences below take 28.1 instead of 26.6 us, the smallest broken calls 0.4 more.)
-    __device__ __forceinline__ bool count_up(int cta, int shift, int count) const {
+    __device__ __forceinline__ bool count_up(int of, int shift, int count) const {
         unsigned int before;
         asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(before)
-                     : "l"(a.arrived + cta), "r"(1u << shift) : "memory");
+                     : "l"(a.arrived + index(of)), "r"(1u << shift) : "memory");
         const bool all = static_cast<int>(before >> shift & (shift == 16 ? 0xffffu : 0xffu)) == count - 1;
-        if (all) atomicSub(a.arrived + cta, static_cast<unsigned int>(count) << shift);
+        if (all) atomicSub(a.arrived + index(of), static_cast<unsigned int>(count) << shift);
         return all;
     }
     // n parts, every `stride` CTAs from `from` on, to `out` (a part's place) or, if that is null, to the result's rows.  The
-    // parts are copied into the ring, then a thread takes some columns of a row, four at a time.  (Little code: it is run once a launch, and
-    // its own way from memory costs more than what it does: with eight parts at a time in registers 4 us.)
-    __device__ __forceinline__ void sum(int first, int from, int stride, int n, float* out, int b, int h, int row0) const {
-        const int size = part_floats(), rows = min(kRows, a.G - row0), cap = C::kRingBytes / 4 / size;
+    // parts are copied into the ring, then a thread takes some columns of a row, four at a time.  (Little code: it is run once
+    // a launch, and its own way from memory costs more than what it does: with eight parts at a time in registers 4 us.)
+    __device__ __forceinline__ void sum(int first, int from, int stride, int n, float* out, int b, int h) const {
+        const int size = part_floats(), rows = min(kRows, a.G - row0()), cap = C::kRingBytes / 4 / size;
         int have = 0;  // 1: the sum so far lies in front
 #pragma unroll 1
         for (int i0 = 0; i0 < n;) {
@@ -333,13 +343,13 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
             const int lane = threadIdx.x & 31;
 #pragma unroll 1
             for (int i = threadIdx.x >> 5; i < add; i += C::kWarps) {
-                const int cta = from + (i0 + i) * stride;
-                const float* const part = a.ws + decode_part_at<D, E8, NT>(cta, cta == first) + lane * 4;
+                const int of = from + (i0 + i) * stride;
+                const float* const src = part(of, of == first) + lane * 4;
                 const uint32_t dst = smem_u32(room + (have + i) * size) + lane * 16;
 #pragma unroll
                 for (int c = 0; c < kRows * (D / 4); c += 32)  // the rows that exist, then maxima and sums
-                    if (c < rows * (D / 4)) cp_async16(dst + c * 16, part + c * 4);
-                if (lane < 2 * kRows / 4) cp_async16(dst + (size - 2 * kRows) * 4, part + kRows * D);
+                    if (c < rows * (D / 4)) cp_async16(dst + c * 16, src + c * 4);
+                if (lane < 2 * kRows / 4) cp_async16(dst + (size - 2 * kRows) * 4, src + kRows * D);
             }
             cp_async_commit();
             cp_async_wait<0>();
@@ -378,7 +388,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                     } else if (out != nullptr) {
                         *reinterpret_cast<float4*>(out + r * D + c * 4 + at) = z[k];
                     } else {
-                        T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + c * 4 + at;
+                        T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0() + r) * a.o_sh + c * 4 + at;
                         *reinterpret_cast<uint2*>(dst) =
                             make_uint2(Num<T>::pack(z[k].x * inv, z[k].y * inv), Num<T>::pack(z[k].z * inv, z[k].w * inv));
                     }
@@ -401,25 +411,23 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     // counts have to go on): count it.  True: the part completes its group.
     __device__ __forceinline__ bool part_done(const DecodeBroken& it) const {
         const int group = join_group(it.last - it.first + 1);
-        const int from = it.first + (static_cast<int>(blockIdx.x) - it.first) / group * group;
+        const int from = it.first + (cta - it.first) / group * group;
         const int n = min(group, it.last - from + 1);
         return n == 1 || count_up(from, from == it.first ? 8 : 0, n);
     }
     // All threads, once, behind the counting: the joins that fall to this CTA (those whose s_flag is set).
     __device__ __forceinline__ void run(const DecodeBroken (&item)[2], bool dead) const {
-        const int cta = blockIdx.x;
 #pragma unroll 1
         for (int k = 0; k < 2; ++k) {
             if (s_flag[k] == 0) continue;
             const DecodeBroken it = k == 0 ? item[0] : item[1];
             const int group = join_group(it.last - it.first + 1), groups = (it.last - it.first) / group + 1;
-            const int row0 = (it.hk - it.h * a.row_blocks) * kRows;
             int from = it.first + (cta - it.first) / group * group, stride = 1, n = min(group, it.last - from + 1);
             bool final = groups == 1;
 #pragma unroll 1
             for (;;) {
-                float* const place = final ? nullptr : a.ws + decode_part_at<D, E8, NT>(from, from == it.first);
-                if (n > 1 && !dead) sum(it.first, from, stride, n, place, it.b, it.h, row0);
+                float* const place = final ? nullptr : part(from, from == it.first);
+                if (n > 1 && !dead) sum(it.first, from, stride, n, place, it.b, it.h);
                 if (final) break;
                 __syncthreads();
                 if (threadIdx.x == 0) s_flag[k] = count_up(it.first, 16, groups);
@@ -442,7 +450,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     constexpr int kDT = D / 16, kRows = C::kRows;
     __shared__ int s_dead, s_flag[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const int HK = a.Hkv * a.row_blocks, n_ctas = gridDim.x;
+    const int n_ctas = gridDim.x / a.row_blocks, cta = blockIdx.x / a.row_blocks, row_block = blockIdx.x - cta * a.row_blocks;
+    const int row0 = row_block * kRows;
     if (tid == 0) s_dead = *reinterpret_cast<volatile int*>(a.status);  // (one reading for the whole CTA)
 
     // ---- this CTA's piece of the line of units; each warp finds it for itself
@@ -466,34 +475,33 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             const unsigned int x = __shfl_up_sync(0xffffffffu, before, d);
             if (lane >= d) before += x;
         }
-        const unsigned int sum = __shfl_sync(0xffffffffu, before, 31), total = sum * HK;  // (the host has seen to it that this fits)
+        const unsigned int sum = __shfl_sync(0xffffffffu, before, 31), total = sum * a.Hkv;  // (the host has seen to it that this fits)
         const unsigned int average = sum / max(__reduce_add_sync(0xffffffffu, rows_at_all), 1u);
         const unsigned int least = average <= kDecWhole / (C::kTiles * (D / 128)) + C::kItemCost ? average : 1 + C::kItemCost;
         piece = max((total + n_ctas - 1) / n_ctas, max(least, 1u));
-        u0 = piece * blockIdx.x;
+        u0 = piece * cta;
         u1 = min(u0 + piece, total);
         before -= mine;
-        const unsigned int here = __ballot_sync(0xffffffffu, u0 < total && before * HK <= u0 && u0 < (before + mine) * HK);
+        const unsigned int here = __ballot_sync(0xffffffffu, u0 < total && before * a.Hkv <= u0 && u0 < (before + mine) * a.Hkv);
         int b = b_lo;
         if (here >> lane & 1) {
             for (;;) {
                 const int rows = cached_rows(a, b);
                 const unsigned int n = rows > 0 ? units_of<C::kUnit>(rows) + C::kItemCost : 0;
-                if (u0 < (before + n) * HK) break;
+                if (u0 < (before + n) * a.Hkv) break;
                 before += n;
                 ++b;
             }
         }
         const int src = here == 0 ? 0 : __ffs(here) - 1;
         cc.b = __shfl_sync(0xffffffffu, b, src);
-        const unsigned int in_b = u0 - __shfl_sync(0xffffffffu, before, src) * HK;
+        const unsigned int in_b = u0 - __shfl_sync(0xffffffffu, before, src) * a.Hkv;
         cc.left = 0;
         if (here != 0) {
             cc.len = cached_rows(a, cc.b);
             cc.nt = units_of<C::kUnit>(cc.len);
-            cc.hk = in_b / (cc.nt + C::kItemCost);
-            cc.t = static_cast<int>(in_b - cc.hk * (cc.nt + C::kItemCost)) - C::kItemCost;
-            cc.h = cc.hk / a.row_blocks;
+            cc.h = in_b / (cc.nt + C::kItemCost);
+            cc.t = static_cast<int>(in_b - cc.h * (cc.nt + C::kItemCost)) - C::kItemCost;
             cc.left = u1 - u0;
             if (cc.t < 0) {  // in front of the item's first unit
                 cc.left += cc.t;
@@ -502,7 +510,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         }
     }
     auto empty_rows = [&] {  // sequences without rows have no units: their output is zero
-        for (int b = blockIdx.x; b < a.B; b += n_ctas)
+        for (int b = blockIdx.x; b < a.B; b += gridDim.x)
             if (cached_rows(a, b) == 0)
                 for (int i = tid; i < a.Hkv * a.G * (D / 8); i += C::kThreads)
                     reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + b * a.o_sb + (i / (D / 8)) * a.o_sh)[i % (D / 8)] =
@@ -514,15 +522,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         return;
     }
     // the broken items: the one that began before this piece (or fills it), and the one that begins in it and goes on
-    DecodeBroken broken[2] = {{-1, 0, 0, 0, 0}, {-1, 0, 0, 0, 0}};
+    DecodeBroken broken[2] = {{-1, 0, 0, 0}, {-1, 0, 0, 0}};
     auto cta_of = [&](unsigned int u) { return static_cast<int>(u / piece); };
     if (cc.t > 0) {
         const unsigned int from = u1 - cc.left - cc.t;  // the item's first unit
-        broken[0] = {cta_of(from), cta_of(from + cc.nt - 1), cc.b, cc.hk, cc.h};
+        broken[0] = {cta_of(from), cta_of(from + cc.nt - 1), cc.b, cc.h};
     }
     auto begins_and_goes_on = [&](int n) {  // n units of item cc are here
         if (cc.t == 0 && n < cc.nt)
-            broken[1] = {static_cast<int>(blockIdx.x), cta_of(u1 - cc.left + cc.nt - 1), cc.b, cc.hk, cc.h};
+            broken[1] = {cta, cta_of(u1 - cc.left + cc.nt - 1), cc.b, cc.h};
     };
 
     // ---- the warp's ring of slots: K rows, V rows, K rows ... of its steps (16-byte pieces xor-ed with the row so that
@@ -539,7 +547,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
 
     QueryRows<D, T, NT, C::kWarps> rows;
     using R = Row<D, 32>;
-    rows.load(a, cc);
+    rows.load(a, cc, row0);
     typename R::Words gamma;
     if (a.gamma != nullptr) R::template load<false>(gamma, a.gamma, lane);
 
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             ++pc.t;
             --pc.left;
             if (pc.t == pc.nt && pc.left > 0) {
-                pc.next_item(a, HK);
+                pc.next_item(a);
                 if (pc.left > 0) {
                     head_sources();
                     look_up();
@@ -655,7 +663,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     };
     auto leave = [&] { slot = slot + 1 == C::kSlots ? 0 : slot + 1; };
 
-    const DecodeJoin<D, T, E8, NT> join{a, reinterpret_cast<float*>(smem), s_flag};
+    const DecodeJoin<D, T, E8, NT> join{a, reinterpret_cast<float*>(smem), s_flag, cta, row_block};
     if (tid == 0) s_flag[0] = s_flag[1] = 0;
     rows.template prepare<E8>(a, gamma, frag, back);
     __syncthreads();
@@ -667,7 +675,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             begins_and_goes_on(n);
             cc.t += n;
             cc.left -= n;
-            if (cc.left > 0) cc.next_item(a, HK);
+            if (cc.left > 0) cc.next_item(a);
         }
         if (tid == 0)
 #pragma unroll 1
@@ -687,7 +695,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         R::template load<false>(kw, reinterpret_cast<const T*>(a.new_k) + cc.b * a.nk_sb + cc.h * a.nk_sh, lane);
         R::template load<false>(vw, reinterpret_cast<const T*>(a.new_v) + cc.b * a.nv_sb + cc.h * a.nv_sh, lane);
         if (a.gamma_k != nullptr) R::template load<false>(gk, a.gamma_k, lane);
-        bool write = cc.hk == cc.h * a.row_blocks && __ldg(a.lengths + cc.b) <= a.c.capacity;
+        bool write = row_block == 0 && __ldg(a.lengths + cc.b) <= a.c.capacity;
         if (a.cos != nullptr) {
             write = write && pos < a.n_pos;
             const long long at = static_cast<long long>(min(pos, a.n_pos - 1)) * D;
@@ -746,12 +754,12 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         // ---- one item's part: units cc.t .. cc.t + n - 1
         const int n = min(cc.nt - cc.t, cc.left);
         if (n <= 0) break;
-        const int h = cc.h, row0 = (cc.hk - h * a.row_blocks) * kRows;
+        const int h = cc.h;
         auto nc = cc;  // the item after this one: its query rows are on their way meanwhile
         nc.t += n;
         nc.left -= n;
-        if (nc.left > 0) nc.next_item(a, HK);
-        if (nc.left > 0) rows.load(a, nc);
+        if (nc.left > 0) nc.next_item(a);
+        if (nc.left > 0) rows.load(a, nc, row0);
         uint4 qf[C::kQueryInRegs ? NT : 1][C::kQueryInRegs ? kDT : 1];
         if constexpr (C::kQueryInRegs) {
 #pragma unroll
@@ -1000,7 +1008,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             }
         const bool whole = n == cc.nt;
         begins_and_goes_on(n);
-        float* const part = a.ws + decode_part_at<D, E8, NT>(blockIdx.x, cc.t == 0 ? 1 : 0);
+        float* const part = join.part(cta, cc.t == 0);
         float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
         // eight rows and kMergeCols columns at a time: the last two warps leave theirs, two after two add theirs, all add the
         // two copies

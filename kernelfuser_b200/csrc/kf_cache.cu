@@ -149,15 +149,16 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
     kf::DecodeArgs args = a;
     args.row_blocks = (a.G + 8 * NT - 1) / (8 * NT);
-    // no more CTAs than the batch can have pieces of work
-    const long long items = static_cast<long long>(a.B) * a.Hkv * args.row_blocks, unit = kf::DecodeCfg<D, E8, NT>::kUnit;
+    // a CTA for each block of query rows of every piece of the line; no more pieces than the batch can have
+    const long long items = static_cast<long long>(a.B) * a.Hkv, unit = kf::DecodeCfg<D, E8, NT>::kUnit;
     const long long per_item = (a.c.capacity + unit - 1) / unit;
     const long long most = items * (per_item + kf::DecodeCfg<D, E8, NT>::kItemCost);
     if (most > 0x7fffffffLL)
         return fail(KF_EINVAL, "the batch is too large: its page table can hold more than 2^31 pieces of 64 keys");
-    const long long fit = decode_ctas<D, E8, NT>();
-    const unsigned grid = (unsigned)(items * per_item < fit ? items * per_item : fit);
-    if (grid > 1) {
+    const long long fit = decode_ctas<D, E8, NT>(), room = fit / args.row_blocks > 0 ? fit / args.row_blocks : 1;
+    const long long pieces = items * per_item < room ? items * per_item : room;
+    const unsigned grid = (unsigned)(pieces * args.row_blocks);
+    if (pieces > 1) {
         if (int r = join_words(st, &args.arrived)) return r;
         if (args.arrived == nullptr) {  // then words in the workspace, cleared by the graph itself
             args.arrived = reinterpret_cast<unsigned int*>(a.ws + kf::decode_part_at<D, E8, NT>((int)fit, 0));

@@ -109,6 +109,22 @@ def test_long_sequences_are_split_and_joined(cache, lengths, hq, hkv, d):
         assert torch.equal(kf.decode_attention(q, p.cache, p.pages, ints(lengths), gq, cos, sin), got)
 
 
+@pytest.mark.parametrize("cache", ["16", "e4m3"])
+@pytest.mark.parametrize("lengths,hq,hkv,d", [
+    ([70, 0, 400], 4800, 1, 128),         # more blocks of 16 query heads than CTAs
+    ([9000, 77], 40, 1, 128),             # the last block half full, broken items
+    ([3000, 1, 0, 801], 100, 2, 256),
+])
+def test_many_query_heads_share_a_step(cache, lengths, hq, hkv, d):
+    p = Paged(lengths, hkv, d, 16, E8 if cache == "e4m3" else BF, seed=91)
+    q, k, v = rand(92, len(lengths), hq, 1, d), rand(93, len(lengths), hkv, 1, d), rand(94, len(lengths), hkv, 1, d)
+    got = kf.decode_step(q, k, v, p.cache, p.pages, ints(lengths))  # (writes the last row, once)
+    again = kf.decode_step(q, k, v, p.cache, p.pages, ints(lengths))
+    done()
+    check(got, *attention(p, q, lengths, None, None, None))
+    assert torch.equal(got, again)
+
+
 def test_more_captured_launches_than_join_words():
     # a captured launch has words of its own to count in, 4096 at a time; a further one gets them from its workspace
     lengths, most = [3000, 70], 4300
