@@ -82,6 +82,11 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     // and have twice as many independent products (64 sequences of 4096 rows, G = 4: 118 -> 98 us, floor 83), and three CTAs
     // give the schedulers a third warp each (135 -> 116 us with steps of 16; four, at 128 registers: 124).
     // With more than eight heads of 256 O alone takes 128 registers and one CTA's queries 16 KB: eight warps share them.
+    // The first pages of the next item are looked up when an item is entered: waiting for them at the border, twice where a
+    // piece begins near an item's end, made the last CTAs late (16 sequences of 8192 rows, 8 heads: 21.5 -> 20.4 us; four of
+    // 8192, 32/8 heads 31.1 -> 30.1).  The 8-bit and the wide kernels have no registers left for it (64 x 4096 rows 94.1 -> 95.7;
+    // 48/2 heads of 256 132 -> 155).
+    static constexpr bool kLookAhead = !E8 && !kWide;
     // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
     static constexpr int kSlots = E8 ? (kWide || (D == 128 && NT == 2) ? 5 : 3) : D == 256 ? 3 : NT == 1 ? 6 : 5;
     // columns that meet at a time; a row of them in shared memory
@@ -601,16 +606,25 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             }
         }
     };
-    // pages of the units from pc.t on; looked at when the next K rows are asked for
+    // this lane's page, and row in it, of the units of an item from `first` on; looked at when K rows are asked for
+    auto page_of = [&](const auto& item, int first, int& row) {
+        const int unit = first + lane / C::kTiles, key = unit * C::kUnit + warp * C::kKeys + lane % C::kTiles * 16;
+        row = 0;
+        if (unit >= item.nt || key >= item.len) return 0;
+        const int i = key / a.c.page_size;
+        row = key - i * a.c.page_size;
+        return __ldg(a.c.pages + item.b * a.c.pages_sb + i);
+    };
     auto look_up = [&] {
         table_at = pc.t;
-        my_page = my_row = 0;
-        const int unit = pc.t + lane / C::kTiles, key = unit * C::kUnit + warp * C::kKeys + lane % C::kTiles * 16;
-        if (unit < pc.nt && key < pc.len) {
-            const int i = key / a.c.page_size;
-            my_row = key - i * a.c.page_size;
-            my_page = __ldg(a.c.pages + pc.b * a.c.pages_sb + i);
-        }
+        my_page = page_of(pc, pc.t, my_row);
+    };
+    int next_page = 0, next_row = 0;  // the first ones of the item after pc's
+    auto look_ahead = [&] {
+        auto next = pc;
+        next.left -= next.nt - next.t;
+        if (next.left > 0) next.next_item(a);
+        if (next.left > 0) next_page = page_of(next, 0, next_row);
     };
     auto issue_k = [&](int slot) {
         if (pc.left > 0) {
@@ -636,7 +650,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                 pc.next_item(a);
                 if (pc.left > 0) {
                     head_sources();
-                    look_up();
+                    if constexpr (C::kLookAhead) {
+                        table_at = 0;
+                        my_page = next_page;
+                        my_row = next_row;
+                        look_ahead();
+                    } else {
+                        look_up();
+                    }
                 }
             } else if (pc.t - table_at == kLook) {
                 look_up();
@@ -646,6 +667,7 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     };
     head_sources();
     look_up();
+    if constexpr (C::kLookAhead) look_ahead();
 #pragma unroll 1
     for (int s = 0; s < C::kSlots - 1; s += 2) {
         issue_k(s);
