@@ -64,6 +64,8 @@ _16 = frozenset(_DTYPES)
 
 def _bad_cache(k, v, ks, vs, pages, b, dtype, index):
     """The error of a cache or table that does not fit."""
+    if k.requires_grad or v.requires_grad:
+        raise ValueError("This API is forward-only")
     if k.ndim != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _CACHE_DTYPES:
         raise ValueError("Expected cache pools [n_pages, Hkv, page_size, D] of one type (BF16, FP16 or float8_e4m3fn)")
     n, h, page, d = k.shape
@@ -92,7 +94,8 @@ def _cache_fields(cache, pages, b, dtype, index):
     e8 = kind is _E8
     ok = (len(shape) == 4 and v.shape == shape and v.dtype is kind and (e8 or kind is dtype) and len(table) == 2 and
           table[0] == b and table[1] >= 1 and pages.dtype is _INT and (sp[1] == 1 or table[1] == 1) and
-          k.get_device() == v.get_device() == pages.get_device() == index >= 0 and sk[3] == 1 == sv[3])
+          k.get_device() == v.get_device() == pages.get_device() == index >= 0 and sk[3] == 1 == sv[3] and
+          not (k.requires_grad or v.requires_grad))
     if ok:
         n, h, page, d = shape
         ok = (d == 128 or d == 256) and n >= 1 and h >= 1 and page >= 16 and page % 16 == 0

@@ -543,6 +543,17 @@ def test_indexes_outside_are_reported_and_nothing_else_is_touched():
     done()
 
 
+def test_a_cache_that_needs_a_gradient_is_refused():
+    p = Paged([5, 9], 2, 128, 16, BF, seed=95)
+    q, n = rand(96, 2, 4, 1, 128), ints([5, 9])
+    for cache in ((p.k.clone().requires_grad_(), p.v), (p.k, p.v.clone().requires_grad_())):
+        for call in (lambda: kf.decode_attention(q, cache, p.pages, n), lambda: kf.read_rows(cache, p.pages, n, 9),
+                     lambda: kf.append_rows(cache, q[:, :2], q[:, :2], p.pages, n)):
+            with pytest.raises(ValueError, match="forward-only"):
+                call()
+    done()
+
+
 def test_offsets_past_32_bits():
     # a pool of more than 2^32 bytes, the sequence in its last pages
     n_pages = (1 << 32) // (64 * 128 * 2) + 40
