@@ -89,12 +89,15 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr bool kLookAhead = !E8 && !kWide;
     // slots of a warp's ring: as many as let that many CTAs onto an SM (about 100 KB each of two)
     static constexpr int kSlots = E8 ? (kWide || (D == 128 && NT == 2) ? 5 : 3) : D == 256 ? 3 : NT == 1 ? 6 : 5;
+    // Copies of O in which the warps meet, one after the other in each (eight warps, 64 sequences of 1000 rows, 32/2 heads of
+    // 256: 40 us with two, 37 with four; for four warps of an 8-bit cache four gained nothing, of a 16-bit one they do not fit).
+    static constexpr int kCopies = kWide ? 4 : 2;
     // columns that meet at a time; a row of them in shared memory
     static constexpr int kMergeCols = D == 256 || E8 ? 64 : 128, kPad = kMergeCols + 4;
     static constexpr int kRingBytes = kWarps * kSlots * kSlotBytes;
     static constexpr int kScaleRingBytes = kWarps * kSlots * kScaleBytes;
     static constexpr int kQueryBytes = NT * (D / 16) * 32 * 16;       // {high, high, low, low} fragments of a lane
-    static constexpr int kMergeBytes = 2 * 8 * kPad * 4 + (2 * kWarps + 1) * kRows * 4;
+    static constexpr int kMergeBytes = kCopies * 8 * kPad * 4 + (2 * kWarps + 1) * kRows * 4;
     static constexpr int kNewBytes = 2 * kRowBytes;                   // a new token's K and V row
     static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes + kNewBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
@@ -544,8 +547,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     const uint32_t ring = smem_u32(smem) + warp * C::kSlots * C::kSlotBytes;
     unsigned char* const scales = smem + C::kSmemBytes - C::kScaleRingBytes + warp * C::kSlots * C::kScaleBytes;
     uint4* const frag = reinterpret_cast<uint4*>(smem + C::kRingBytes);
-    float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes + C::kQueryBytes);  // two copies of [8][kPad]
-    float* const merge_m = merge_o + 2 * 8 * C::kPad;                                        // [warps][rows]
+    float* const merge_o = reinterpret_cast<float*>(smem + C::kRingBytes + C::kQueryBytes);  // kCopies of [8][kPad]
+    float* const merge_m = merge_o + C::kCopies * 8 * C::kPad;                               // [warps][rows]
     float* const merge_l = merge_m + C::kWarps * kRows;
     float* const back = merge_l + C::kWarps * kRows;                                         // [rows]
     unsigned char* const new_rows = smem + C::kSmemBytes - C::kScaleRingBytes - C::kNewBytes;  // K and V row of a new token
@@ -1031,9 +1034,9 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
         const bool whole = n == cc.nt;
         begins_and_goes_on(n);
         float* const part = join.part(cta, cc.t == 0);
-        float* const copy = merge_o + (warp & 1) * 8 * C::kPad;
-        // eight rows and kMergeCols columns at a time: the last two warps leave theirs, two after two add theirs, all add the
-        // two copies
+        float* const copy = merge_o + warp % C::kCopies * 8 * C::kPad;
+        // eight rows and kMergeCols columns at a time: the last kCopies warps leave theirs, the ones before add theirs, all add the
+        // copies
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -1046,21 +1049,24 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                             f((2 * t4 + (k & 1)) * C::kPad + 16 * i + (E8 ? 2 * g + (k >> 1) : g + 8 * (k >> 1)),
                               o[u][c0 / 16 + i][k]);
                 };
-                if (warp >= C::kWarps - 2) each([&](int at, float x) { copy[at] = x; });
+                if (warp >= C::kWarps - C::kCopies) each([&](int at, float x) { copy[at] = x; });
                 __syncthreads();
                 // (all are done with the old ones)
                 if (u == 0 && c0 == 0 && nc.left > 0) rows.template prepare<E8>(a, gamma, frag, back);
 #pragma unroll 1
-                for (int w = C::kWarps - 4; w >= 0; w -= 2) {
-                    if ((warp & ~1) == w) each([&](int at, float x) { copy[at] += x; });
+                for (int w = C::kWarps - 2 * C::kCopies; w >= 0; w -= C::kCopies) {
+                    if (warp / C::kCopies * C::kCopies == w) each([&](int at, float x) { copy[at] += x; });
                     __syncthreads();
                 }
                 for (int i = tid; i < 8 * (C::kMergeCols / 4); i += C::kThreads) {
                     const int r8 = i / (C::kMergeCols / 4), d8 = (i % (C::kMergeCols / 4)) * 4, r = u * 8 + r8, d = c0 + d8;
                     if (row0 + r >= a.G) break;  // (rows go up with i)
-                    const float4 x = *reinterpret_cast<const float4*>(merge_o + r8 * C::kPad + d8);
-                    const float4 y = *reinterpret_cast<const float4*>(merge_o + (8 + r8) * C::kPad + d8);
-                    const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+                    float4 z = *reinterpret_cast<const float4*>(merge_o + r8 * C::kPad + d8);
+#pragma unroll
+                    for (int i = 1; i < C::kCopies; ++i) {
+                        const float4 y = *reinterpret_cast<const float4*>(merge_o + (8 * i + r8) * C::kPad + d8);
+                        z = make_float4(z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w);
+                    }
                     float top = -INFINITY, sum = 0.f;
 #pragma unroll
                     for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
