@@ -100,7 +100,7 @@ template <int D, bool E8, int NT> struct DecodeCfg {
     static constexpr int kMergeBytes = kCopies * 8 * kPad * 4 + (2 * kWarps + 1) * kRows * 4;
     static constexpr int kNewBytes = 2 * kRowBytes;                   // a new token's K and V row
     static constexpr int kSmemBytes = kRingBytes + kQueryBytes + kMergeBytes + kScaleRingBytes + kNewBytes;
-    static constexpr int kPartFloats = kRows * D + 2 * kRows;         // output, maximum, sum of a broken item
+    static constexpr int kPartFloats = kRows * D + 2 * kRows;         // mean, and its weight, of a broken item's part
 };
 
 // Copies of cache rows into shared memory.  Each row is read once, so it is the first to leave L2 again: what is read over and
@@ -304,6 +304,16 @@ struct DecodeBroken {
     int b, h;
 };
 
+// A part is the mean of its value rows and their weight, mantissa * 2^exponent: what a sum of probabilities against a base comes
+// to, with the mantissa brought to [2^-8, 2^-7).  The weighted parts of a join, 64 at most, then add up to less than the largest
+// value: it may be as large as 32 bits hold.  (0, infinity and NaN stay.)
+__device__ __forceinline__ void part_weight(float* exponent, float* mantissa, float base, float sum) {
+    const int e = static_cast<int>(__float_as_uint(sum) >> 23) - 119;
+    const bool plain = sum > 0.f && sum < INFINITY;
+    *exponent = plain ? base + static_cast<float>(e) : base;
+    *mantissa = plain ? __uint_as_float((__float_as_uint(sum) & 0x7fffffu) | 119u << 23) : sum;
+}
+
 template <int D, typename T, bool E8, int NT> struct DecodeJoin {
     using C = DecodeCfg<D, E8, NT>;
     static constexpr int kRows = C::kRows;
@@ -355,7 +365,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                 const float* const src = part(of, of == first) + lane * 4;
                 const uint32_t dst = smem_u32(room + (have + i) * size) + lane * 16;
 #pragma unroll
-                for (int c = 0; c < kRows * (D / 4); c += 32)  // the rows that exist, then maxima and sums
+                for (int c = 0; c < kRows * (D / 4); c += 32)  // the rows that exist, then their weights
                     if (c < rows * (D / 4)) cp_async16(dst + c * 16, src + c * 4);
                 if (lane < 2 * kRows / 4) cp_async16(dst + (size - 2 * kRows) * 4, src + kRows * D);
             }
@@ -366,7 +376,7 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
             // a thread stays in one row, so that it takes the row's weights once
             const int shift = __clz(rows - 1) - __clz(C::kThreads) - 1;  // 2^shift threads to a row
             const int r = static_cast<int>(threadIdx.x) >> shift, c = threadIdx.x & ((1 << shift) - 1);
-            float* const m = room + size - 2 * kRows + r;  // of the first part
+            float* const m = room + size - 2 * kRows + r;  // exponents of the first part's weights; mantissas kRows further
             float top = -INFINITY, total = 0.f;
             if (r < rows && c < D / 4) {
 #pragma unroll 4
@@ -377,8 +387,8 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                 float* const row = room + r * D + c * 4;
 #pragma unroll 2
                 for (int i = 0; i < count; ++i) {
-                    const float mi = m[i * size], w = mi == -INFINITY ? 0.f : ex2(mi - top);
-                    total = fmaf(m[i * size + kRows], w, total);
+                    const float mi = m[i * size], w = m[i * size + kRows] * (mi == -INFINITY ? 0.f : ex2(mi - top));
+                    total += w;
 #pragma unroll
                     for (int k = 0; k < kQuads; ++k) {
                         if (c + (k << shift) >= D / 4) break;
@@ -386,11 +396,13 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                         z[k] = make_float4(fmaf(x.x, w, z[k].x), fmaf(x.y, w, z[k].y), fmaf(x.z, w, z[k].z), fmaf(x.w, w, z[k].w));
                     }
                 }
-                const float inv = 1.f / total;
+                // (no weight at all: undefined, and as a part nothing)
+                const float inv = total != 0.f ? 1.f / total : i0 >= n && out == nullptr ? NAN : 0.f;
 #pragma unroll
                 for (int k = 0; k < kQuads; ++k) {
                     const int at = (k << shift) * 4;
                     if (c * 4 + at >= D) break;
+                    z[k] = make_float4(z[k].x * inv, z[k].y * inv, z[k].z * inv, z[k].w * inv);
                     if (i0 < n) {
                         *reinterpret_cast<float4*>(row + at) = z[k];  // (what only this thread has read)
                     } else if (out != nullptr) {
@@ -398,17 +410,16 @@ template <int D, typename T, bool E8, int NT> struct DecodeJoin {
                     } else {
                         T* const dst = reinterpret_cast<T*>(a.out) + b * a.o_sb + (h * a.G + row0() + r) * a.o_sh + c * 4 + at;
                         *reinterpret_cast<uint2*>(dst) =
-                            make_uint2(Num<T>::pack(z[k].x * inv, z[k].y * inv), Num<T>::pack(z[k].z * inv, z[k].w * inv));
+                            make_uint2(Num<T>::pack(z[k].x, z[k].y), Num<T>::pack(z[k].z, z[k].w));
                     }
                 }
             }
             if (i0 >= n && out == nullptr) break;
-            // maximum and sum of the rows, once all have read the old ones
+            // weights of the rows, once all have read the old ones
             __syncthreads();
             if (r < rows && c == 0) {
                 float* const to = i0 < n ? m : out + kRows * D + r;
-                to[0] = top;
-                to[kRows] = total;
+                part_weight(to, to + kRows, top, total);
             }
             have = 1;
             __syncthreads();
@@ -1016,22 +1027,36 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                 }
             }
         __syncthreads();
+        const bool whole = n == cc.nt;
+        auto top_and_sum = [&](int r, float& top, float& sum) {  // of row r over the warps
+            top = -INFINITY;
+            sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
+#pragma unroll
+            for (int w = 0; w < C::kWarps; ++w) {
+                const float lw = merge_l[w * kRows + r];
+                sum += lw == 0.f ? 0.f : lw * ex2(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
+            }
+        };
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + u * 8 + 2 * t4 + c]);
-                const float f = mv[u][c] == -INFINITY ? 0.f : ex2(mv[u][c] - (top == -INFINITY ? 0.f : top));
-                // (a warp without keys has a zero output; one whose scores are all -inf keeps a NaN that it may hold)
+                float top, sum;
+                top_and_sum(u * 8 + 2 * t4 + c, top, sum);
+                // Divided by the sum before it is brought to the common base: that step gives an 8-bit cache's values their scale
+                // back (up to 2^127), and what is added up from then on is at most the largest of them.  (In two halves, as
+                // the factor itself may be more than 32 bits hold.  No weight at all: the whole item is undefined, a part counts
+                // for nothing.)
+                const float half = mv[u][c] == -INFINITY ? 0.f : ex2(0.5f * (mv[u][c] - top));
+                const float f = (sum != 0.f ? 1.f / sum : whole ? NAN : 0.f) * half;
 #pragma unroll
                 for (int i = 0; i < kDT; ++i) {
-                    o[u][i][c] = f == 0.f && o[u][i][c] == 0.f ? 0.f : o[u][i][c] * f;
-                    o[u][i][c + 2] = f == 0.f && o[u][i][c + 2] == 0.f ? 0.f : o[u][i][c + 2] * f;
+                    o[u][i][c] = o[u][i][c] * f * half;
+                    o[u][i][c + 2] = o[u][i][c + 2] * f * half;
                 }
             }
-        const bool whole = n == cc.nt;
         begins_and_goes_on(n);
         float* const part = join.part(cta, cc.t == 0);
         float* const copy = merge_o + warp % C::kCopies * 8 * C::kPad;
@@ -1067,24 +1092,15 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                         const float4 y = *reinterpret_cast<const float4*>(merge_o + (8 * i + r8) * C::kPad + d8);
                         z = make_float4(z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w);
                     }
-                    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-                    for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
-#pragma unroll
-                    for (int w = 0; w < C::kWarps; ++w) {
-                        const float lw = merge_l[w * kRows + r];
-                        sum += lw == 0.f ? 0.f : lw * ex2(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
-                    }
                     if (whole) {
                         T* const dst = reinterpret_cast<T*>(a.out) + cc.b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
-                        const float inv = 1.f / sum;
-                        *reinterpret_cast<uint2*>(dst) =
-                            make_uint2(Num<T>::pack(z.x * inv, z.y * inv), Num<T>::pack(z.z * inv, z.w * inv));
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x, z.y), Num<T>::pack(z.z, z.w));
                     } else {
                         *reinterpret_cast<float4*>(part + r * D + d) = z;
                         if (d == 0) {
-                            part[kRows * D + r] = top;
-                            part[kRows * D + kRows + r] = sum;
+                            float top, sum;
+                            top_and_sum(r, top, sum);
+                            part_weight(part + kRows * D + r, part + kRows * D + kRows + r, top, sum);
                         }
                     }
                 }
