@@ -781,10 +781,11 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     const uint32_t v_lane = ring + v_row * C::kRowBytes + ((v_piece ^ (v_row & 7)) << 4);
     auto step32 = [](uint32_t at, int j) { return (at ^ ((j & 3) << 5)) + (j >> 2) * 128; };
     // Probabilities are 2^(score - base + kUp), the base at most kSlack behind the largest score so far: up to 2^15 in f16,
-    // whose smallest step is then 2^-35 of the largest probability, up to 2^8 in bf16.
+    // whose smallest step is then 2^-35 of the largest probability, up to 2^-12 in bf16, so that a warp's sum over 4096 of
+    // the largest bf16 values is still finite (values below 2^-106 lose bits for it).
     constexpr bool kHalf = std::is_same<M, __half>::value;
     constexpr bool kSplit = kSplitProducts<T, E8>;
-    constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : 0.f;
+    constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : -20.f;
 
     while (cc.left > 0) {
         // ---- one item's part: units cc.t .. cc.t + n - 1

@@ -69,3 +69,17 @@ def test_a_large_value_row_that_a_step_appends():
     torch.cuda.synchronize()
     kf.check_status()
     check(got, *attention_close(p, q, lengths, None, cos, sin))
+
+
+@pytest.mark.parametrize("power", [127, 122, -90])
+@pytest.mark.parametrize("lengths", LENGTHS)
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (16, 1, 128), (2, 1, 256), (11, 1, 256)])
+def test_values_at_the_ends_of_bf16(power, lengths, hq, hkv, d):
+    # below 2^power, and half of them near it: the result is a mean of them, whatever their sum
+    p = Paged(lengths, hkv, d, 16, BF, seed=79)
+    p.v.clamp_(-0.99, 0.99).mul_(2.0 ** power)
+    q = rand(80, len(lengths), hq, 1, d)
+    got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+    torch.cuda.synchronize()
+    kf.check_status()
+    check(got, *attention_close(p, q, lengths, None, None, None))
