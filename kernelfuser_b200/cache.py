@@ -301,4 +301,6 @@ def decode_step(q, k, v, cache, pages, lengths, gq=None, gk=None, cos=None, sin=
     """One generated token of every sequence: its ``k`` and ``v`` [B, Hkv, 1, D] are appended at position
     ``lengths[b] - 1`` (as ``append_rows`` does) and its query attends to all ``lengths[b]`` rows (``decode_attention``).
     ``lengths`` counts the new token; a sequence with ``lengths[b] <= 0`` appends nothing and gets zeros."""
+    if k is None or v is None:  # (without rows it would be decode_attention, over a row that nothing has written)
+        raise ValueError("Expected K/V [B,Hkv,1,D]: one token per sequence")
     return _decode(q, k, v, cache, pages, lengths, gq, gk, cos, sin, eps, scale, out, workspace)
