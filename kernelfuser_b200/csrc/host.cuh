@@ -156,29 +156,58 @@ template <int N> struct GraphSlots {
     }
 };
 
-// The slot of the launch about to be made into `st`: one of the first `eager` in turn (two launches could only share one if
-// one were still running when that many later ones have been started), or, while the stream is being captured, one of SLOTS
-// behind them; -1 when every one of those is taken.
-template <auto& SLOTS> int launch_slot(cudaStream_t st, std::atomic<unsigned int>& turn, int eager, int* out) {
+// Slots that launches into streams use: one for each stream, as launches of one stream never run at the same time, while those
+// of two may, however far apart they were enqueued (one may wait for an event while thousands go through the other).  A stream is
+// known by its context's and its own number, which are never used again in a process.  (Plain data.)
+template <int N> struct StreamSlots {
+    std::atomic_flag busy = ATOMIC_FLAG_INIT;
+    unsigned long long context[N], stream[N];  // context 0: nobody's slot
+    int of(unsigned long long ctx, unsigned long long id) {  // -1: every slot belongs to another stream
+        const unsigned int first = static_cast<unsigned int>((ctx * 31 + id) * 2654435761u >> 7) % N;
+        while (busy.test_and_set(std::memory_order_acquire)) {}
+        int at = -1;
+        for (int i = 0; i < N && at < 0; ++i) {
+            const int k = static_cast<int>((first + i) % N);
+            if (context[k] == 0) {
+                context[k] = ctx;
+                stream[k] = id;
+            }
+            if (context[k] == ctx && stream[k] == id) at = k;
+        }
+        busy.clear(std::memory_order_release);
+        return at;
+    }
+};
+
+// The slot of the launch about to be made into `st`: its stream's, or, while the stream is being captured, one of GRAPH's behind
+// all of those; -1 when every slot of the kind is taken, or the stream cannot be told from others.
+template <auto& STREAM, auto& GRAPH> int launch_slot(cudaStream_t st, int* out) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     cudaGraph_t graph = nullptr;
     if (cudaStreamGetCaptureInfo_v2(st, &capture, nullptr, &graph, nullptr, nullptr) != cudaSuccess) {
         cudaGetLastError();  // (the legacy stream next to a capture elsewhere: the launch itself reports that)
         capture = cudaStreamCaptureStatusNone;
     }
+    *out = -1;
     if (capture != cudaStreamCaptureStatusActive) {
-        *out = static_cast<int>(turn.fetch_add(1, std::memory_order_relaxed) % static_cast<unsigned int>(eager));
+        const unsigned long long ctx = context_id();
+        unsigned long long id = 0;
+        if (ctx == 0) return KF_OK;
+        if (cudaStreamGetId(st, &id) != cudaSuccess) {
+            cudaGetLastError();
+            return KF_OK;
+        }
+        *out = STREAM.of(ctx, id);
         return KF_OK;
     }
-    *out = -1;
-    const int slot = SLOTS.take();
+    const int slot = GRAPH.take();
     if (slot < 0) return KF_OK;
     cudaUserObject_t owner = nullptr;
     cudaError_t e = cudaUserObjectCreate(&owner, reinterpret_cast<void*>(static_cast<intptr_t>(slot)),
-                                         [](void* tag) { SLOTS.give_back(static_cast<int>(reinterpret_cast<intptr_t>(tag))); }, 1,
+                                         [](void* tag) { GRAPH.give_back(static_cast<int>(reinterpret_cast<intptr_t>(tag))); }, 1,
                                          cudaUserObjectNoDestructorSync);
     if (e != cudaSuccess) {
-        SLOTS.give_back(slot);
+        GRAPH.give_back(slot);
         return fail(KF_ECUDA, "cudaUserObjectCreate failed: %s", cudaGetErrorString(e));
     }
     e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
@@ -186,7 +215,7 @@ template <auto& SLOTS> int launch_slot(cudaStream_t st, std::atomic<unsigned int
         cudaUserObjectRelease(owner, 1);  // (gives the slot back)
         return fail(KF_ECUDA, "cudaGraphRetainUserObject failed: %s", cudaGetErrorString(e));
     }
-    *out = eager + slot;
+    *out = static_cast<int>(sizeof(STREAM.stream) / sizeof(STREAM.stream[0])) + slot;
     return KF_OK;
 }
 

@@ -208,24 +208,24 @@ constexpr long long kAutoPersistMinTiles = 8192;
 constexpr int kAutoPersistMinS = 2048, kAutoPersistMaxS = 8192;
 
 // Work counters of the persistent kernels: {next item, CTAs that have left}, zero between launches (in the library image;
-// the last CTA of a launch puts them back).  Launches into a stream take the first kSchedSlots in turn, so two could only
-// share one if a launch were still running when that many later ones have been started.  A captured launch runs again
-// with every replay of its graph, next to whatever else is running: it gets one of the other kGraphSlots for itself,
-// which the graph, its clones and its executable forms own together and give back when the last of them is destroyed.
+// the last CTA of a launch puts them back).  Each stream has one of the first kSchedSlots, as its launches run one after the
+// other.  A captured launch runs again with every replay of its graph, next to whatever else is running: it gets one of the
+// other kGraphSlots for itself, which the graph, its clones and its executable forms own together and give back when the last
+// of them is destroyed.
 constexpr int kSchedSlots = 1024, kGraphSlots = 1 << 14;
 __device__ unsigned int g_sched[kSchedSlots + kGraphSlots][2];
 
+StreamSlots<kSchedSlots> g_sched_slots;
 GraphSlots<kGraphSlots> g_sched_graph_slots;
 
-// The counters of the launch about to be made into `st`; NULL: it is being captured and every graph slot is taken.
+// The counters of the launch about to be made into `st`; NULL: every slot is taken.
 int sched_slot(cudaStream_t st, unsigned int** out) {
     static SymbolCache cache;
-    static std::atomic<unsigned int> turn{0};
     void* p = nullptr;
     cudaError_t e = symbol_address(cache, g_sched, &p);
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(work counters) failed: %s", cudaGetErrorString(e));
     int slot = -1;
-    if (int r = launch_slot<g_sched_graph_slots>(st, turn, kSchedSlots, &slot)) return r;
+    if (int r = launch_slot<g_sched_slots, g_sched_graph_slots>(st, &slot)) return r;
     *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + 2 * slot;
     return KF_OK;
 }

@@ -118,21 +118,20 @@ template <int D, typename T, bool E8> int launch_read(const kf::ReadArgs& a, cud
 }
 
 // Words in which the CTAs of a decode launch count what has arrived for a join: a row of them per launch, zero between
-// launches (in the library image; the CTA that completes a count takes it back).  Launches into a stream take the first
-// kJoinSlots rows in turn, a captured one has one of its own.
+// launches (in the library image; the CTA that completes a count takes it back).  Each stream has a row, and each captured launch.
 constexpr int kMaxCtas = 512, kJoinSlots = 1024, kJoinGraphSlots = 4096;
 __device__ unsigned int g_arrived[kJoinSlots + kJoinGraphSlots][kMaxCtas];
+StreamSlots<kJoinSlots> g_join_slots;
 GraphSlots<kJoinGraphSlots> g_join_graph_slots;
 
-// NULL: the launch is being captured and every graph slot is taken.
+// NULL: every row is taken.
 int join_words(cudaStream_t st, unsigned int** out) {
     static SymbolCache cache;
-    static std::atomic<unsigned int> turn{0};
     void* p = nullptr;
     cudaError_t e = symbol_address(cache, g_arrived, &p);
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(join words) failed: %s", cudaGetErrorString(e));
     int slot = -1;
-    if (int r = launch_slot<g_join_graph_slots>(st, turn, kJoinSlots, &slot)) return r;
+    if (int r = launch_slot<g_join_slots, g_join_graph_slots>(st, &slot)) return r;
     *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + static_cast<size_t>(slot) * kMaxCtas;
     return KF_OK;
 }
@@ -160,7 +159,7 @@ template <int D, typename T, bool E8, int NT> int launch_decode_nt(const kf::Dec
     const unsigned grid = (unsigned)(pieces * args.row_blocks);
     if (pieces > 1) {
         if (int r = join_words(st, &args.arrived)) return r;
-        if (args.arrived == nullptr) {  // then words in the workspace, cleared by the graph itself
+        if (args.arrived == nullptr) {  // then words in the workspace, cleared first
             args.arrived = reinterpret_cast<unsigned int*>(a.ws + kf::decode_part_at<D, E8, NT>((int)fit, 0));
             e = cudaMemsetAsync(args.arrived, 0, sizeof(unsigned int) * grid, st);
             if (e != cudaSuccess) return fail(KF_ECUDA, "cudaMemsetAsync failed: %s", cudaGetErrorString(e));
