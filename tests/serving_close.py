@@ -10,6 +10,11 @@ from serving import U, transform
 LEFT = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22}
 SMS = 148
 
+# (lengths, Hq, Hkv, D) of launches whose items are broken over CTAs, or whole and of many steps
+LONG = [([70001], 8, 1, 128), ([9000, 1, 0, 5000, 13], 4, 2, 128), ([20000, 64], 2, 1, 256), ([4097] * 3, 16, 1, 256),
+        ([6000, 700], 24, 1, 128), ([900] * 150, 24, 1, 128), ([1500] * 150, 16, 1, 256), ([1300] * 300, 2, 1, 256),
+        ([2100] * 450, 3, 1, 128), ([900] * 40, 8, 4, 128)]
+
 
 def steps_of(lengths, hkv, n):
     """Products in a row that a warp of four adds to its output for a sequence of n keys: of 16 keys each, 64 keys a round.  A
@@ -65,3 +70,22 @@ def attention_close(paged, q, lengths, gamma, cos, sin, scale=None, only=None):
         out[i, :, 0] = o
         bound[i, :, 0] = e + (o.abs() + e) * U[q.dtype] + (2.0 ** -25 if q.dtype == torch.float16 else 2.0 ** -134)
     return out, bound
+
+
+def region_values(paged, lengths):
+    """Value rows that say where in the sequence they stand: row p of n holds a one in column p * D // n and zeros, so that column c
+    of the result is the weight of one D-th of the sequence.  (An e4m3 cache: scale 1.)"""
+    d = paged.v.shape[-1]
+    for b, n in enumerate(lengths):
+        if n <= 0:
+            continue
+        pages = -(-n // paged.page)
+        col = (torch.arange(pages * paged.page, device=paged.v.device) * d // n).clamp_max(d - 1)
+        rows = torch.zeros(pages * paged.page, d, device=paged.v.device).scatter_(1, col[:, None], 1.0).to(paged.v.dtype)
+        at, rows = paged.pages[b, :pages].long(), rows.view(pages, 1, paged.page, d).expand(-1, paged.v.shape[1], -1, -1)
+        if paged.v_scale is None:
+            paged.v[at] = rows
+        else:
+            paged.v.view(torch.uint8)[at] = rows.contiguous().view(torch.uint8)
+    if paged.v_scale is not None:
+        paged.v_scale.view(torch.uint8).fill_(127)
