@@ -781,8 +781,8 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
     const uint32_t v_lane = ring + v_row * C::kRowBytes + ((v_piece ^ (v_row & 7)) << 4);
     auto step32 = [](uint32_t at, int j) { return (at ^ ((j & 3) << 5)) + (j >> 2) * 128; };
     // Probabilities are 2^(score - base + kUp), the base at most kSlack behind the largest score so far: up to 2^15 in f16,
-    // whose smallest step is then 2^-35 of the largest probability, up to 2^-12 in bf16, so that a warp's sum over 4096 of
-    // the largest bf16 values is still finite (values below 2^-106 lose bits for it).
+    // whose smallest step is then 2^-35 of the largest probability, up to 2^-12 in bf16, so that a sum over 4096 of the
+    // largest bf16 values is still finite (values below 2^-106 lose bits for it).
     constexpr bool kHalf = std::is_same<M, __half>::value;
     constexpr bool kSplit = kSplitProducts<T, E8>;
     constexpr float kSlack = kHalf ? 4.f : 8.f, kUp = kHalf ? 11.f : -20.f;
@@ -1029,34 +1029,38 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
             }
         __syncthreads();
         const bool whole = n == cc.nt;
-        auto top_and_sum = [&](int r, float& top, float& sum) {  // of row r over the warps
-            top = -INFINITY;
-            sum = 0.f;
+        auto top_of = [&](int r) {  // base of row r over the warps
+            float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < C::kWarps; ++w) top = fmaxf(top, merge_m[w * kRows + r]);
+            return top;
+        };
+        auto sum_of = [&](int r, float top) {
+            float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < C::kWarps; ++w) {
                 const float lw = merge_l[w * kRows + r];
                 sum += lw == 0.f ? 0.f : lw * ex2(merge_m[w * kRows + r] - (top == -INFINITY ? 0.f : top));
             }
+            return sum;
         };
+        // what makes means of sums; no weight at all: the whole item is undefined, a part counts for nothing
+        auto inverse = [&](float sum) { return sum != 0.f ? 1.f / sum : whole ? NAN : 0.f; };
 #pragma unroll
         for (int u = 0; u < NT; ++u)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top, sum;
-                top_and_sum(u * 8 + 2 * t4 + c, top, sum);
-                // Divided by the sum before it is brought to the common base: that step gives an 8-bit cache's values their scale
-                // back (up to 2^127), and what is added up from then on is at most the largest of them.  (In two halves, as
-                // the factor itself may be more than 32 bits hold.  No weight at all: the whole item is undefined, a part counts
-                // for nothing.)
-                const float half = mv[u][c] == -INFINITY ? 0.f : ex2(0.5f * (mv[u][c] - top));
-                const float f = (sum != 0.f ? 1.f / sum : whole ? NAN : 0.f) * half;
+                const int r = u * 8 + 2 * t4 + c;
+                const float top = top_of(r), by = mv[u][c] - (top == -INFINITY ? 0.f : top);
+                // To the common base.  That gives an 8-bit cache's values their scale back (up to 2^127), so they are divided by the
+                // sum first: what is added up from then on is at most the largest value.  (In two halves, as the factor itself
+                // may be more than 32 bits hold.)
+                const float f = mv[u][c] == -INFINITY ? 0.f : ex2(E8 ? 0.5f * by : by);
+                const float first = E8 ? f * inverse(sum_of(r, top)) : f;
 #pragma unroll
-                for (int i = 0; i < kDT; ++i) {
-                    o[u][i][c] = o[u][i][c] * f * half;
-                    o[u][i][c + 2] = o[u][i][c + 2] * f * half;
-                }
+                for (int i = 0; i < kDT; ++i)
+#pragma unroll
+                    for (int k = c; k < 4; k += 2) o[u][i][k] = E8 ? o[u][i][k] * first * f : o[u][i][k] * f;
             }
         begins_and_goes_on(n);
         float* const part = join.part(cta, cc.t == 0);
@@ -1093,16 +1097,14 @@ __global__ void __launch_bounds__(DecodeCfg<D, E8, NT>::kThreads, DecodeCfg<D, E
                         const float4 y = *reinterpret_cast<const float4*>(merge_o + (8 * i + r8) * C::kPad + d8);
                         z = make_float4(z.x + y.x, z.y + y.y, z.z + y.z, z.w + y.w);
                     }
+                    const float top = top_of(r), sum = sum_of(r, top), inv = E8 ? 1.f : inverse(sum);
+                    z = make_float4(z.x * inv, z.y * inv, z.z * inv, z.w * inv);
                     if (whole) {
                         T* const dst = reinterpret_cast<T*>(a.out) + cc.b * a.o_sb + (h * a.G + row0 + r) * a.o_sh + d;
                         *reinterpret_cast<uint2*>(dst) = make_uint2(Num<T>::pack(z.x, z.y), Num<T>::pack(z.z, z.w));
                     } else {
                         *reinterpret_cast<float4*>(part + r * D + d) = z;
-                        if (d == 0) {
-                            float top, sum;
-                            top_and_sum(r, top, sum);
-                            part_weight(part + kRows * D + r, part + kRows * D + kRows + r, top, sum);
-                        }
+                        if (d == 0) part_weight(part + kRows * D + r, part + kRows * D + kRows + r, top, sum);
                     }
                 }
                 __syncthreads();  // the copies are free
