@@ -78,14 +78,16 @@ template <auto KERN> cudaError_t allow_smem(int bytes) {
     return e;
 }
 
-// Device address, in the current context, of a variable of the library image; looked up once per context.
+// Device address, in the current context, of a variable of the library image; looked up once per context.  And the context's
+// number.
 struct SymbolCache {
     std::atomic_flag busy = ATOMIC_FLAG_INIT;
     unsigned long long id[64];
     void* at[64];
 };
-inline cudaError_t symbol_address(SymbolCache& c, const void* symbol, void** out) {
-    const unsigned long long id = context_id();
+inline cudaError_t symbol_address(SymbolCache& c, const void* symbol, void** out,
+                                  unsigned long long* context = nullptr) {
+    unsigned long long id = context_id();
     const int i = static_cast<int>(id % 64);
     auto locked = [&](auto&& body) {
         while (c.busy.test_and_set(std::memory_order_acquire)) {}
@@ -97,10 +99,11 @@ inline cudaError_t symbol_address(SymbolCache& c, const void* symbol, void** out
     if (p == nullptr) {
         cudaError_t e = cudaGetSymbolAddress(&p, symbol);
         if (e != cudaSuccess) return e;
-        if (const unsigned long long now = context_id())  // (the call may have made the context)
-            locked([&] { c.id[now % 64] = now; c.at[now % 64] = p; });
+        id = context_id();  // (the call may have made the context)
+        if (id != 0) locked([&] { c.id[id % 64] = id; c.at[id % 64] = p; });
     }
     *out = p;
+    if (context != nullptr) *context = id;
     return cudaSuccess;
 }
 
@@ -179,9 +182,9 @@ template <int N> struct StreamSlots {
     }
 };
 
-// The slot of the launch about to be made into `st`: its stream's, or, while the stream is being captured, one of GRAPH's behind
+// The slot of the launch about to be made into `st` in context `ctx`: its stream's, or, while the stream is being captured, one of GRAPH's behind
 // all of those; -1 when every slot of the kind is taken, or the stream cannot be told from others.
-template <auto& STREAM, auto& GRAPH> int launch_slot(cudaStream_t st, int* out) {
+template <auto& STREAM, auto& GRAPH> int launch_slot(cudaStream_t st, unsigned long long ctx, int* out) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     cudaGraph_t graph = nullptr;
     if (cudaStreamGetCaptureInfo_v2(st, &capture, nullptr, &graph, nullptr, nullptr) != cudaSuccess) {
@@ -190,7 +193,6 @@ template <auto& STREAM, auto& GRAPH> int launch_slot(cudaStream_t st, int* out) 
     }
     *out = -1;
     if (capture != cudaStreamCaptureStatusActive) {
-        const unsigned long long ctx = context_id();
         unsigned long long id = 0;
         if (ctx == 0) return KF_OK;
         if (cudaStreamGetId(st, &id) != cudaSuccess) {

@@ -222,10 +222,11 @@ GraphSlots<kGraphSlots> g_sched_graph_slots;
 int sched_slot(cudaStream_t st, unsigned int** out) {
     static SymbolCache cache;
     void* p = nullptr;
-    cudaError_t e = symbol_address(cache, g_sched, &p);
+    unsigned long long context = 0;
+    cudaError_t e = symbol_address(cache, g_sched, &p, &context);
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(work counters) failed: %s", cudaGetErrorString(e));
     int slot = -1;
-    if (int r = launch_slot<g_sched_slots, g_sched_graph_slots>(st, &slot)) return r;
+    if (int r = launch_slot<g_sched_slots, g_sched_graph_slots>(st, context, &slot)) return r;
     *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + 2 * slot;
     return KF_OK;
 }

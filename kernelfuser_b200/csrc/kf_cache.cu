@@ -128,10 +128,11 @@ GraphSlots<kJoinGraphSlots> g_join_graph_slots;
 int join_words(cudaStream_t st, unsigned int** out) {
     static SymbolCache cache;
     void* p = nullptr;
-    cudaError_t e = symbol_address(cache, g_arrived, &p);
+    unsigned long long context = 0;
+    cudaError_t e = symbol_address(cache, g_arrived, &p, &context);
     if (e != cudaSuccess) return fail(KF_ECUDA, "cudaGetSymbolAddress(join words) failed: %s", cudaGetErrorString(e));
     int slot = -1;
-    if (int r = launch_slot<g_join_slots, g_join_graph_slots>(st, &slot)) return r;
+    if (int r = launch_slot<g_join_slots, g_join_graph_slots>(st, context, &slot)) return r;
     *out = slot < 0 ? nullptr : static_cast<unsigned int*>(p) + static_cast<size_t>(slot) * kMaxCtas;
     return KF_OK;
 }
