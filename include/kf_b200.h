@@ -212,7 +212,9 @@ int kf_selftest_wait_timeout(int* status, long long limit_clocks, void* stream);
  *
  * K rows and queries go through RMSNorm (gamma; NULL: none) and the split-half
  * rotation (cos/sin [n_positions, D]; NULL for both: none) in 32 bits and are
- * rounded once, to the cache's type (K) or the type of the products (Q).
+ * rounded once, to the cache's type (K), or kept as two 16-bit numbers (Q), as
+ * the probabilities are: 2^-16 (bf16) or 2^-22 (fp16) of a value is left.  With
+ * bf16 q and a KF_E4M3 cache both are one f16 number, off by up to 2^-12.
  *
  * What the lengths and tables on the device hold cannot be checked on the
  * host.  A kernel that meets a table entry outside the cache writes 911 into

@@ -13,6 +13,14 @@ K rows and queries are normed (``gk`` / ``gq``; None: not) and rotated (``cos`` 
 fp32 and rounded once; ``optimized_attention`` rounds at every step of its reference's contract, so rows that have to equal
 its ``kn`` bit for bit are appended from ``kn``, with ``gk`` and the tables left out.
 
+Attention sums in fp32.  Prepared queries and probabilities enter its products as two 16-bit numbers each, which leaves 2^-16
+(bf16) or 2^-22 (fp16) of a value; in a bf16 call on an e4m3 cache as ONE f16 number, off by 2^-12 of it or less, an eighth of
+what rounding the result to bf16 costs.
+
+The layout that decoding reads fastest is the one of ``PagedCache.allocate``, rows of a head D apart.  Any pool with contiguous
+rows is taken, [n_pages, page_size, Hkv, D] viewed as [n_pages, Hkv, page_size, D] among them, but copied row by row: long
+16-bit sequences take the same time from it, a ragged step of 32 short ones a sixth more, an e4m3 cache a quarter more.
+
 Lengths and tables on the device are not looked at by the host.  A table entry outside the cache, a length or position
 that the table cannot hold or one behind the rotary tables is reported through the status word (``check_status`` raises);
 nothing is read or written out of bounds.

@@ -192,8 +192,8 @@ constexpr int kRowsThreads = 256;
 
 // A group of D/16 lanes takes up to kAppendHeads heads of one position, so that the tables are read once for them and their
 // rows are in flight together; K rows and V rows are different CTAs' work (blockIdx.z).  Bound by HBM (16 bits: 16384 rows
-// of eight heads in 26.5 us = 5.1 TB/s; one head in flight 33, K and V in one lane 43) and by the latency of a CTA's chain
-// of loads: 80 registers, three CTAs an SM (e4m3 30.5 -> 26.7 us).
+// of eight heads in 27.3 us = 5.0 TB/s, launches in a graph; one head in flight 33, K and V in one lane 43) and by the latency
+// of a CTA's chain of loads: 80 registers, three CTAs an SM (e4m3 30.5 -> 27.1 us).
 constexpr int kAppendHeads = 4;
 
 template <int D, typename T, bool E8>
