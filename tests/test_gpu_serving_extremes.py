@@ -83,3 +83,70 @@ def test_values_at_the_ends_of_bf16(power, lengths, hq, hkv, d):
     torch.cuda.synchronize()
     kf.check_status()
     check(got, *attention_close(p, q, lengths, None, None, None))
+
+
+# (len, heads): whole items of many steps; one item over every CTA, joined in groups; a few parts joined at once
+BROKEN = [([900] * 150, 4), ([70001], 4), ([70001], 16), ([9000, 13, 5000], 8)]
+
+
+def minus_infinite_keys(p, b, first, last):
+    """Keys first .. last-1 of sequence b whose scores are -inf for queries with a one in column 0."""
+    at = torch.arange(first, last, device="cuda")
+    page, row = p.pages[b].long()[at // p.page], at % p.page
+    p.k[page, :, row] = 0
+    p.k[page, :, row, 0] = -float("inf")
+
+
+@pytest.mark.parametrize("lengths,hq", BROKEN)
+def test_parts_without_any_weight(lengths, hq):
+    # keys of whole CTAs' pieces score -inf: the rest alone counts; if all do, nothing is defined
+    p = Paged(lengths, 1, 128, 16, BF, seed=81)
+    q = rand(82, len(lengths), hq, 1, 128)
+    q[..., 0] = 1.0
+    n = lengths[0]
+    for first, last in ((0, n // 2), (n // 2, n - 1), (1, n // 2)):
+        clean = p.k.clone()
+        minus_infinite_keys(p, 0, first, last)
+        got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+        torch.cuda.synchronize()
+        kf.check_status()
+        keep = [r for r in range(n) if not first <= r < last]
+        cut = Paged.__new__(Paged)
+        cut.__dict__.update(p.__dict__)
+        cut.rows = lambda name, b, m: p.rows(name, 0, n)[:, keep]
+        want, bound = attention_close(cut, q[:1], [len(keep)], None, None, None)
+        assert torch.isfinite(got.double()).all()
+        assert ((got[:1].double() - want).abs() <= bound).all()
+        p.k.copy_(clean)
+    minus_infinite_keys(p, 0, 0, n)
+    got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+    torch.cuda.synchronize()
+    kf.check_status()
+    assert torch.isnan(got[0]).all() and torch.isfinite(got[1:].double()).all()
+
+
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("cache", ["16", "e4m3"])
+@pytest.mark.parametrize("lengths,hq", BROKEN)
+def test_nan_and_infinity_in_one_part(lengths, hq, cache, what):
+    p = Paged(lengths, 1, 128, 16, E8 if cache == "e4m3" else BF, seed=83)
+    q, n = rand(84, len(lengths), hq, 1, 128), lengths[0]
+    clean = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+    page, row = int(p.pages[0, (n - 100) // 16]), (n - 100) % 16
+    if cache == "e4m3":
+        getattr(p, what + "_scale").view(torch.uint8)[page, 0, row] = 255
+    else:
+        getattr(p, what)[page, 0, row] = float("nan")
+    got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+    torch.cuda.synchronize()
+    kf.check_status()
+    assert torch.isnan(got[0]).all() and torch.equal(got[1:], clean[1:])
+    if cache == "16" and what == "v":  # an infinity stays in its column
+        getattr(p, what)[page, 0, row] = 1.0
+        clean = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+        p.v[page, 0, row, 5], p.v[page, 0, row, 9] = float("inf"), -float("inf")
+        got = kf.decode_attention(q, p.cache, p.pages, ints(lengths))
+        torch.cuda.synchronize()
+        assert (got[0, ..., 5] == float("inf")).all() and (got[0, ..., 9] == -float("inf")).all()
+        keep = [c for c in range(128) if c not in (5, 9)]
+        assert torch.equal(got[..., keep], clean[..., keep]) and torch.equal(got[1:], clean[1:])
