@@ -34,8 +34,8 @@
 // relative), and the products wait for HBM anyway (see kSplitProducts for the one exception).  Scores, sums and outputs are 32
 // bits.  An e4m3 cache is widened to f16 (exact) on the way into the product; q' is scaled there by a power of two per head so
 // that its largest value is between 2^14 and 2^15; a key's scale multiplies its score, and a value row's scale goes into the
-// exponent of its probability, whose base for O is kept apart from the one for the sum.  What is finite in the cache gives a
-// finite result: warps and parts meet as means of value rows, never as sums of e4m3 rows with their scales.
+// exponent of its probability, whose base for O is kept apart from the one for the sum.  Its warps and parts meet as means of
+// value rows, never as sums of rows with their scales: finite value rows give a finite result (bf16 ones: see kUp).
 #pragma once
 #include <type_traits>
 #include <utility>
